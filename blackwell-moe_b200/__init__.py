@@ -8,8 +8,8 @@ hand-written sm_100a CUDA kernels in ``libbwmoe.so`` reached through a C ABI
 missing or no B200 is present the calls raise.
 """
 
-from .quant import (FP8_MAX_E4M3, dequant_fp8_e4m3, quant_fp8_block_128, quant_fp8_e4m3, quantize_expert_weights,
-                    quantize_expert_weights_block)
+from .quant import (FP8_MAX_E4M3, dequant_fp8_e4m3, quant_fp8_block_128, quant_fp8_e4m3, quant_int8_channels,
+                    quantize_expert_weights, quantize_expert_weights_block, quantize_expert_weights_int8)
 from .moe import (
     HostPipeline,
     fp8_moe_forward,
@@ -21,6 +21,9 @@ from .moe import (
     streaming_moe_forward,
     top_k_router,
 )
+from .permute import PermutePlan, permute_plan, permute_tokens, unpermute_tokens, unpermute_tokens_backward
+from .int8 import (int8_grouped_gemm, int8_grouped_swiglu, int8_matmul, int8_moe_forward, int8_moe_forward_routed,
+                   quantize_tokens_int8)
 from ._lib import lib, library_path, BwmoeError
 from .modules import (FP8MixtralSparseMoeBlock, FP8MoELayer, FP8SharedExpert, fp8_dense_mlp,
                       patch_deepseek_moe_with_store, patch_shared_experts)
@@ -40,4 +43,7 @@ __all__ = [
     "fp8_moe_forward_small_e", "fp8_moe_forward_v3", "fp8_moe_forward_v4", "lib", "library_path",
     "moe_stage_views", "quant_fp8_block_128", "quant_fp8_e4m3", "quantize_expert_weights",
     "quantize_expert_weights_block", "top_k_router",
+    "PermutePlan", "permute_plan", "permute_tokens", "unpermute_tokens", "unpermute_tokens_backward",
+    "int8_grouped_gemm", "int8_grouped_swiglu", "int8_matmul", "int8_moe_forward", "int8_moe_forward_routed",
+    "quant_int8_channels", "quantize_expert_weights_int8", "quantize_tokens_int8",
 ]

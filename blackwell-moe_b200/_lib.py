@@ -80,6 +80,19 @@ SIGNATURES = {
                                            C.POINTER(C.c_void_p), _i, _i, _ip, _vp]),
     "bwmoe_scatter_quant_peers": (_i, [_vp, _ip, _ip, _fp, _ip, _i, _i, _i, _i, C.POINTER(C.c_void_p), _i, _i, _ip,
                                        _vp]),
+    "bwmoe_permute_tokens": (_i, [_vp, _ip] + [_i] * 5 + [_ip] * 4 + [_vp, _ip, _vp, _vp]),
+    "bwmoe_permute_rows": (_i, [_vp, _ip, _ip] + [_i] * 5 + [_vp, _vp]),
+    "bwmoe_unpermute_rows": (_i, [_vp, _ip, _fp] + [_i] * 4 + [_vp, _vp]),
+    "bwmoe_unpermute_rows_backward": (_i, [_vp, _vp, _ip, _ip, _fp] + [_i] * 5 + [_vp, _fp, _vp]),
+    "bwmoe_int_quant": (_i, [_vp, _ip, _ip] + [_i] * 5 + [_vp, _fp, _vp]),
+    "bwmoe_int_scratch_bytes": (_sz, [_i] * 4),
+    "bwmoe_int_grouped_gemm": (_i, [_vp, _fp, _ip, _vp, _fp] + [_i] * 5 + [_vp, _vp, _sz, _vp]),
+    "bwmoe_int_gateup_swiglu": (_i, [_vp, _fp, _ip, _vp, _vp, _fp, _fp] + [_i] * 5 + [_vp, _vp, _sz, _vp]),
+    "bwmoe_workspace_bytes_int_matmul": (_sz, [_i] * 3),
+    "bwmoe_int_matmul": (_i, [_vp, _vp, _fp] + [_i] * 4 + [_vp, _vp, _sz, _vp]),
+    "bwmoe_workspace_bytes_int": (_sz, [_i] * 5),
+    "bwmoe_moe_forward_int_routed": (_i, [_vp, _fp, _ip] + [_vp] * 3 + [_fp] * 3 + [_i] * 6 + [_vp, _vp, _sz, _vp]),
+    "bwmoe_moe_forward_int": (_i, [_vp] * 5 + [_fp] * 3 + [_i] * 5 + [_vp, _vp, _sz, _vp]),
     "bwmoe_combine_peers": (_i, [C.POINTER(C.c_void_p), _i, _ip, _ip, _fp, _ip, _i, _i, _i, _i, _vp, _vp]),
 }
 

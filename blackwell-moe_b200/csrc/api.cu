@@ -316,6 +316,95 @@ int check_block_args(const char* who, const void* x, const void* wg, const void*
   return BWMOE_OK;
 }
 
+// Workspace of the block over experts in 8-bit integers.  The first block is cleared at the start of a call.
+struct Int8Layout {
+  size_t status, gemm_scratch, zero_end, offsets, topk_idx, topk_w, pos, row_slot, row_expert, plan_scratch;
+  size_t router_head, router_scratch, router_scratch_bytes, xq, sx, h, hq, sh, y, total;
+};
+
+bool make_int8_layout(int T, int D, int H, int E, int K, Int8Layout* L) {
+  if (T <= 0 || D <= 0 || H <= 0 || E <= 0 || K <= 0 || D % 16 != 0 || H % 16 != 0 || E > 256 || K > E || K > 32) return false;
+  if ((long long)T * K >= (1ll << 31) || std::max(D, H) >= (1 << 17)) return false;
+  const size_t M = (size_t)T * K;
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = o;
+    o = align_up(o + bytes);
+    return at;
+  };
+  L->status = take(16);
+  L->router_head = take(kRouterHeadBytes);
+  L->zero_end = o;
+  L->gemm_scratch = take(int8_scratch_bytes((int)M, std::max(D, H), std::max(D, H), E));
+  L->offsets = take(sizeof(int32_t) * (E + 1));
+  L->topk_idx = take(sizeof(int32_t) * M);
+  L->topk_w = take(sizeof(float) * M);
+  L->pos = take(sizeof(int32_t) * M);
+  L->row_slot = take(sizeof(int32_t) * M);
+  L->row_expert = take(sizeof(int32_t) * M);
+  L->plan_scratch = take(plan_scratch_bytes(T, E, K));
+  L->xq = take(M * D);
+  L->sx = take(sizeof(float) * M);
+  L->h = take(M * H * 2);
+  L->hq = take(M * H);
+  L->sh = take(sizeof(float) * M);
+  L->y = take(M * D * 2);
+  L->router_scratch_bytes = router_scratch_bytes(T, D, E, K);
+  L->router_scratch = take(L->router_scratch_bytes);
+  L->total = o;
+  return true;
+}
+
+int check_int8_args(const char* who, const void* x, const void* wg, const void* wu, const void* wd, const float* sg,
+                    const float* su, const float* sd, int T, int D, int H, int E, int K, int dtype, void* out, void* ws,
+                    size_t ws_bytes, Int8Layout* L) {
+  BWMOE_REQUIRE(T > 0 && D > 0 && H > 0 && E > 0 && K > 0, BWMOE_ERR_BAD_SHAPE, "%s: T=%d D=%d H=%d E=%d K=%d", who, T, D, H,
+                E, K);
+  BWMOE_REQUIRE(D % 16 == 0 && H % 16 == 0, BWMOE_ERR_BAD_SHAPE, "%s: D=%d and H=%d must be multiples of 16", who, D, H);
+  BWMOE_REQUIRE(E <= 256, BWMOE_ERR_UNSUPPORTED, "%s: E=%d > 256 experts", who, E);
+  BWMOE_REQUIRE(K <= E && K <= 32, BWMOE_ERR_UNSUPPORTED, "%s: top_k=%d must be <= min(E,32)", who, K);
+  BWMOE_REQUIRE(dtype == BWMOE_BF16 || dtype == BWMOE_F16, BWMOE_ERR_UNSUPPORTED, "%s: activations are bf16 or fp16", who);
+  BWMOE_REQUIRE(x && wg && wu && wd && sg && su && sd && out, BWMOE_ERR_NULL, "%s: null pointer", who);
+  BWMOE_REQUIRE(make_int8_layout(T, D, H, E, K, L), BWMOE_ERR_BAD_SHAPE, "%s: shape not representable", who);
+  BWMOE_REQUIRE(ws != nullptr && ws_bytes >= L->total, BWMOE_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed",
+                who, ws_bytes, L->total);
+  BWMOE_REQUIRE(aligned16(x) && aligned16(out) && aligned16(wg) && aligned16(wu) && aligned16(wd) && aligned16(sg) &&
+                    aligned16(su) && aligned16(sd) && (reinterpret_cast<uintptr_t>(ws) % 256 == 0),
+                BWMOE_ERR_BAD_ALIGN, "%s: tensors must be 16-byte and the workspace 256-byte aligned", who);
+  return BWMOE_OK;
+}
+
+int run_int8_pipeline(const void* x, const float* weights, const int32_t* indices, const void* wg, const void* wu,
+                      const void* wd, const float* sg, const float* su, const float* sd, int T, int D, int H, int E, int K,
+                      int dtype, void* out, void* ws, const Int8Layout& L, cudaStream_t st) {
+  const int M = T * K;
+  int32_t* status = at<int32_t>(ws, L.status);
+  int32_t *offsets = at<int32_t>(ws, L.offsets), *pos = at<int32_t>(ws, L.pos);
+  float *sx = at<float>(ws, L.sx), *sh = at<float>(ws, L.sh);
+  int rc;
+  if ((rc = launch_plan(indices, nullptr, T, E, K, offsets, pos, at<int32_t>(ws, L.row_slot), at<int32_t>(ws, L.row_expert),
+                        nullptr, status, at<void>(ws, L.plan_scratch), st)))
+    return rc;
+  if ((rc = launch_quant_int8_rows(x, pos, offsets, T, D, E, K, dtype, at<void>(ws, L.xq), sx, st))) return rc;
+  if ((rc = launch_int8_gemm(at<void>(ws, L.xq), sx, offsets, wg, wu, sg, su, M, D, H, E, dtype, at<void>(ws, L.h), status, st)))
+    return rc;
+  if ((rc = launch_quant_int8_rows(at<void>(ws, L.h), nullptr, nullptr, M, H, 1, 1, dtype, at<void>(ws, L.hq), sh, st)))
+    return rc;
+  if ((rc = launch_int8_gemm(at<void>(ws, L.hq), sh, offsets, wd, nullptr, sd, nullptr, M, H, D, E, dtype, at<void>(ws, L.y),
+                             status, st)))
+    return rc;
+  return launch_unpermute_rows(at<void>(ws, L.y), pos, weights, T, D, K, dtype, out, st);
+}
+
+int check_int8_scratch(const char* who, int M, int K, int N, int E, const void* scratch, size_t bytes) {
+  BWMOE_REQUIRE(M > 0 && K > 0 && N > 0 && E > 0, BWMOE_ERR_BAD_SHAPE, "%s: M=%d K=%d N=%d E=%d", who, M, K, N, E);
+  const size_t need = int8_scratch_bytes(M, K, N, E);
+  BWMOE_REQUIRE(scratch != nullptr && bytes >= need, BWMOE_ERR_WORKSPACE, "%s: scratch of %zu bytes given, %zu needed", who, bytes,
+                need);
+  BWMOE_REQUIRE(aligned16(scratch), BWMOE_ERR_BAD_ALIGN, "%s: the scratch must be 16-byte aligned", who);
+  return BWMOE_OK;
+}
+
 }  // namespace
 }  // namespace bwmoe
 
@@ -785,6 +874,118 @@ int bwmoe_combine_peers(void* const* y_of_rank, int n_ranks, const int32_t* pos,
 int bwmoe_combine(const void* y, const int32_t* pos, const float* weights, int T, int D, int K, void* out,
                   void* stream) {
   return launch_combine(y, pos, weights, T, D, K, out, static_cast<cudaStream_t>(stream));
+}
+
+int bwmoe_permute_tokens(const void* x, const int32_t* indices, int T, int D, int E, int K, int dtype, int32_t* offsets,
+                         int32_t* pos, int32_t* row_slot, int32_t* row_expert, void* rows, int32_t* status, void* scratch,
+                         void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  BWMOE_REQUIRE(x && rows, BWMOE_ERR_NULL, "permute_tokens: null pointer");
+  BWMOE_REQUIRE(D > 0 && K <= 32 && dtype >= BWMOE_BF16 && dtype <= BWMOE_F32, BWMOE_ERR_UNSUPPORTED,
+                "permute_tokens: D=%d K=%d type %d", D, K, dtype);
+  BWMOE_REQUIRE((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows)) % dtype_bytes(dtype) == 0, BWMOE_ERR_BAD_ALIGN,
+                "permute_tokens: a pointer is not aligned to its type");
+  if (int rc = launch_plan(indices, nullptr, T, E, K, offsets, pos, row_slot, row_expert, nullptr, status, scratch, st)) return rc;
+  return launch_permute_rows(x, pos, offsets, T, D, E, K, dtype, rows, st);
+}
+
+int bwmoe_permute_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype, void* rows,
+                       void* stream) {
+  return launch_permute_rows(x, pos, offsets, T, D, E, K, dtype, rows, static_cast<cudaStream_t>(stream));
+}
+
+int bwmoe_unpermute_rows(const void* rows, const int32_t* pos, const float* weights, int T, int D, int K, int dtype, void* out,
+                         void* stream) {
+  return launch_unpermute_rows(rows, pos, weights, T, D, K, dtype, out, static_cast<cudaStream_t>(stream));
+}
+
+int bwmoe_unpermute_rows_backward(const void* dout, const void* rows, const int32_t* pos, const int32_t* offsets,
+                                  const float* weights, int T, int D, int E, int K, int dtype, void* drows, float* dweights,
+                                  void* stream) {
+  return launch_unpermute_rows_backward(dout, rows, pos, offsets, weights, T, D, E, K, dtype, drows, dweights,
+                                        static_cast<cudaStream_t>(stream));
+}
+
+int bwmoe_int_quant(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype, void* codes,
+                     float* scales, void* stream) {
+  return launch_quant_int8_rows(x, pos, offsets, T, D, E, K, dtype, codes, scales, static_cast<cudaStream_t>(stream));
+}
+
+size_t bwmoe_int_scratch_bytes(int M, int K, int N, int E) {
+  if (M <= 0 || K <= 0 || N <= 0 || E <= 0) return 0;
+  return int8_scratch_bytes(M, K, N, E);
+}
+
+int bwmoe_int_grouped_gemm(const void* codes, const float* row_scale, const int32_t* offsets, const void* w, const float* scale,
+                            int M, int K, int N, int E, int dtype, void* out, void* scratch, size_t scratch_bytes, void* stream) {
+  if (int rc = check_int8_scratch("int_grouped_gemm", M, K, N, E, scratch, scratch_bytes)) return rc;
+  return launch_int8_gemm(codes, row_scale, offsets, w, nullptr, scale, nullptr, M, K, N, E, dtype, out,
+                          static_cast<int32_t*>(scratch), static_cast<cudaStream_t>(stream), true);
+}
+
+int bwmoe_int_gateup_swiglu(const void* codes, const float* row_scale, const int32_t* offsets, const void* wg, const void* wu,
+                             const float* sg, const float* su, int M, int K, int N, int E, int dtype, void* h, void* scratch,
+                             size_t scratch_bytes, void* stream) {
+  if (int rc = check_int8_scratch("int_gateup_swiglu", M, K, N, E, scratch, scratch_bytes)) return rc;
+  BWMOE_REQUIRE(wu != nullptr, BWMOE_ERR_NULL, "int_gateup_swiglu: null pointer");
+  return launch_int8_gemm(codes, row_scale, offsets, wg, wu, sg, su, M, K, N, E, dtype, h, static_cast<int32_t*>(scratch),
+                          static_cast<cudaStream_t>(stream), true);
+}
+
+size_t bwmoe_workspace_bytes_int_matmul(int T, int K, int N) {
+  if (T <= 0 || K <= 0 || N <= 0 || K % 16 != 0 || N % 16 != 0) return 0;
+  return align_up(int8_scratch_bytes(T, K, N, 1)) + align_up((size_t)T * K) + align_up(sizeof(float) * (size_t)T);
+}
+
+int bwmoe_int_matmul(const void* x, const void* w, const float* scale, int T, int K, int N, int dtype, void* out, void* ws,
+                      size_t ws_bytes, void* stream) {
+  const size_t need = bwmoe_workspace_bytes_int_matmul(T, K, N);
+  BWMOE_REQUIRE(need != 0, BWMOE_ERR_BAD_SHAPE, "int_matmul: T=%d K=%d N=%d (K and N multiples of 16)", T, K, N);
+  BWMOE_REQUIRE(ws != nullptr && ws_bytes >= need, BWMOE_ERR_WORKSPACE, "int_matmul: workspace of %zu bytes given, %zu needed",
+                ws_bytes, need);
+  BWMOE_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0, BWMOE_ERR_BAD_ALIGN, "int_matmul: the workspace must be 256-byte aligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t codes = align_up(int8_scratch_bytes(T, K, N, 1)), scales = codes + align_up((size_t)T * K);
+  if (int rc = check_int8_gemm(at<void>(ws, codes), at<float>(ws, scales), nullptr, w, nullptr, scale, nullptr, T, K, N, 1, dtype, out,
+                               at<int32_t>(ws, 0)))
+    return rc;
+  if (int rc = launch_quant_int8_rows(x, nullptr, nullptr, T, K, 1, 1, dtype, at<void>(ws, codes), at<float>(ws, scales), st, ws, 16))
+    return rc;
+  return launch_int8_gemm(at<void>(ws, codes), at<float>(ws, scales), nullptr, w, nullptr, scale, nullptr, T, K, N, 1, dtype, out,
+                          at<int32_t>(ws, 0), st);
+}
+
+size_t bwmoe_workspace_bytes_int(int T, int D, int H, int E, int K) {
+  Int8Layout L;
+  return make_int8_layout(T, D, H, E, K, &L) ? L.total : 0;
+}
+
+int bwmoe_moe_forward_int_routed(const void* x, const float* weights, const int32_t* indices, const void* wg, const void* wu,
+                                  const void* wd, const float* sg, const float* su, const float* sd, int T, int D, int H, int E,
+                                  int K, int dtype, void* out, void* ws, size_t ws_bytes, void* stream) {
+  Int8Layout L;
+  if (int rc = check_int8_args("moe_forward_int_routed", x, wg, wu, wd, sg, su, sd, T, D, H, E, K, dtype, out, ws, ws_bytes, &L))
+    return rc;
+  BWMOE_REQUIRE(weights && indices, BWMOE_ERR_NULL, "moe_forward_int_routed: routing is null");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  BWMOE_CUDA_OK(cudaMemsetAsync(ws, 0, L.zero_end, st));
+  return run_int8_pipeline(x, weights, indices, wg, wu, wd, sg, su, sd, T, D, H, E, K, dtype, out, ws, L, st);
+}
+
+int bwmoe_moe_forward_int(const void* x, const void* w_gate, const void* wg, const void* wu, const void* wd, const float* sg,
+                           const float* su, const float* sd, int T, int D, int H, int E, int K, void* out, void* ws,
+                           size_t ws_bytes, void* stream) {
+  Int8Layout L;
+  if (int rc = check_int8_args("moe_forward_int", x, wg, wu, wd, sg, su, sd, T, D, H, E, K, BWMOE_BF16, out, ws, ws_bytes, &L))
+    return rc;
+  BWMOE_REQUIRE(w_gate != nullptr, BWMOE_ERR_NULL, "moe_forward_int: w_gate is null");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* weights = at<float>(ws, L.topk_w);
+  int32_t* indices = at<int32_t>(ws, L.topk_idx);
+  if (int rc = launch_router(x, w_gate, T, D, E, K, weights, indices, nullptr, st, at<void>(ws, L.router_scratch),
+                             L.router_scratch_bytes, at<int32_t>(ws, L.status), 0, 0, ws, L.zero_end, at<void>(ws, L.router_head)))
+    return rc;
+  return run_int8_pipeline(x, weights, indices, wg, wu, wd, sg, su, sd, T, D, H, E, K, BWMOE_BF16, out, ws, L, st);
 }
 
 }  // extern "C"

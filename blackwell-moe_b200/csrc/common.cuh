@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -73,6 +74,8 @@ inline cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+inline size_t dtype_bytes(int dtype) { return dtype == BWMOE_F32 ? 4 : 2; }
+template <class T> struct TypeTag { using type = T; };
 int sm_count();
 int gemm_sm_budget();   // sm_count() minus the SMs reserved through bwmoe_set_sm_reserve
 
@@ -281,6 +284,27 @@ int launch_scatter_rows_group_peers(const void* xq_tok, const float* inv_tok, co
                                     const int32_t* indices, const int32_t* delta, int T, int D, int K,
                                     int experts_per_rank, void* const* xq_of_rank, void* const* inv_of_rank,
                                     int n_ranks, int rows_cap, int32_t* status, cudaStream_t st);
+
+// Tokens into expert order and back (permute_rows.cu)
+int launch_permute_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
+                        void* rows, cudaStream_t st);
+int launch_unpermute_rows(const void* rows, const int32_t* pos, const float* weights, int T, int D, int K, int dtype, void* out,
+                          cudaStream_t st);
+int launch_unpermute_rows_backward(const void* dout, const void* rows, const int32_t* pos, const int32_t* offsets,
+                                   const float* weights, int T, int D, int E, int K, int dtype, void* drows, float* dweights,
+                                   cudaStream_t st);
+
+// Experts in 8-bit integers (quant_int8.cu, grouped_gemm_int8_sm100.cu).  zero: words to be cleared on the way.
+int launch_quant_int8_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
+                           void* codes, float* scales, cudaStream_t st, void* zero = nullptr, size_t zero_bytes = 0);
+size_t int8_scratch_bytes(int M, int K, int N, int E);
+// w1 == nullptr: one product; otherwise SwiGLU of the two.  offsets == nullptr: one segment (E = 1).
+int check_int8_gemm(const void* a, const float* row_scale, const int32_t* offsets, const void* w0, const void* w1,
+                    const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, const void* out,
+                    const int32_t* status);
+int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offsets, const void* w0, const void* w1,
+                     const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, void* out, int32_t* status,
+                     cudaStream_t st, bool clear_status = false);
 
 // Monotone map of a float onto unsigned integers (a < b  <=>  key(a) < key(b); -0 is folded onto +0 first).
 __device__ __forceinline__ unsigned order_key(float v) {

@@ -1,0 +1,330 @@
+// Tokens into expert order and back, with gradients.  M = T * K rows; pos[t,k] is the row of slot (t,k), -1 where the
+// slot's expert id was out of range, and the rows offsets[E] .. M-1 then belong to no slot.
+//
+//   permute            rows[pos[t,k]] = x[t]                             its gradient:  dx[t] = sum_k drows[pos[t,k]]
+//   unpermute          out[t] = sum_k w[t,k] * rows[pos[t,k]]            (w absent: 1)
+//   unpermute backward drows[pos[t,k]] = w[t,k] * dout[t]                dw[t,k] = < rows[pos[t,k]], dout[t] >
+//
+// Sums are held in fp32 and added in the order of k (of the row's vectors, for dw), so results do not depend on the
+// launch's timing; a 16-bit result is rounded once.  All of it is bound by memory: every kernel walks the batch by
+// token, so that the token's side (x, out, dout) moves once and only the rows move K times.  Rows that no slot owns are
+// written as zeros.
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace bwmoe {
+namespace {
+
+constexpr int kThreads = 256;
+
+// A row is moved in pieces of 16 bytes; of 8, 4 or 2 where its length or a pointer allows no more.
+template <int BYTES> struct Piece;
+template <> struct Piece<16> { using type = uint4; };
+template <> struct Piece<8> { using type = uint2; };
+template <> struct Piece<4> { using type = uint32_t; };
+template <> struct Piece<2> { using type = uint16_t; };
+
+template <class T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+
+template <class T, int BYTES>
+union Values {
+  typename Piece<BYTES>::type raw;
+  T v[BYTES / sizeof(T)];
+  __device__ Values() {}
+};
+
+template <class P> __device__ __forceinline__ P zero_piece() {
+  P z;
+  memset(&z, 0, sizeof(P));
+  return z;
+}
+
+// Row of slot s; -1 where there is none.  A plan is data from outside the kernel: an entry past the rows is no row.
+__device__ __forceinline__ int row_of(const int32_t* __restrict__ pos, long long s, int M) {
+  const int p = pos[s];
+  return (unsigned)p < (unsigned)M ? p : -1;
+}
+
+// `lanes` threads (a power of two) stand side by side on one token's row, each with U pieces.
+template <int BYTES>
+__global__ void __launch_bounds__(kThreads)
+permute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ x, const int32_t* __restrict__ pos,
+                    const int32_t* __restrict__ offsets, int E, int T, int K, int pieces, int lanes,
+                    typename Piece<BYTES>::type* __restrict__ rows) {
+  using P = typename Piece<BYTES>::type;
+  constexpr int U = 2;
+  chain_wait();
+  const int t = blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes, c0 = blockIdx.y * lanes * U + threadIdx.x % lanes;
+  if (t >= T) return;
+  P v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (c0 + u * lanes < pieces) v[u] = x[(size_t)t * pieces + c0 + u * lanes];
+  const int M = T * K, n_rows = offsets[E];
+#pragma unroll 4
+  for (int k = 0; k < K; ++k) {
+    const int s = t * K + k, p = row_of(pos, s, M);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * lanes;
+      if (c >= pieces) continue;
+      if (p >= 0) rows[(size_t)p * pieces + c] = v[u];
+      if (s >= n_rows) rows[(size_t)s * pieces + c] = zero_piece<P>();
+    }
+  }
+}
+
+// Eight rows at a time: their places first, then their pieces, all requested before the first is used.
+template <class T, int BYTES, bool WEIGHTED>
+__global__ void __launch_bounds__(kThreads)
+unpermute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ rows, const int32_t* __restrict__ pos,
+                      const float* __restrict__ weights, int n_tok, int K, int pieces, int lanes,
+                      typename Piece<BYTES>::type* __restrict__ out) {
+  constexpr int W = BYTES / (int)sizeof(T), R = 8;
+  chain_wait();
+  const int t = blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes, c = blockIdx.y * lanes + threadIdx.x % lanes;
+  if (t >= n_tok || c >= pieces) return;
+  const int M = n_tok * K;
+  float acc[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) acc[i] = 0.f;
+  for (int k0 = 0; k0 < K; k0 += R) {
+    int p[R];
+    float w[R];
+    Values<T, BYTES> q[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      p[j] = k0 + j < K ? row_of(pos, (size_t)t * K + k0 + j, M) : -1;
+      w[j] = WEIGHTED && k0 + j < K ? weights[(size_t)t * K + k0 + j] : 1.f;
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (p[j] >= 0) q[j].raw = rows[(size_t)p[j] * pieces + c];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if (p[j] < 0) continue;
+#pragma unroll
+      for (int i = 0; i < W; ++i) acc[i] = WEIGHTED ? fmaf(w[j], to_f32(q[j].v[i]), acc[i]) : acc[i] + to_f32(q[j].v[i]);
+    }
+  }
+  Values<T, BYTES> o;
+#pragma unroll
+  for (int i = 0; i < W; ++i) o.v[i] = from_f32<T>(acc[i]);
+  out[(size_t)t * pieces + c] = o.raw;
+}
+
+// wpt warps (1, 2, 4 or 8) share a token; lane l of them takes every (32 * wpt)-th piece of the row.
+template <class T, int BYTES, bool DROWS, bool DW>
+__global__ void __launch_bounds__(kThreads)
+unpermute_rows_backward_kernel(const typename Piece<BYTES>::type* __restrict__ dout,
+                               const typename Piece<BYTES>::type* __restrict__ rows, const int32_t* __restrict__ pos,
+                               const int32_t* __restrict__ offsets, int E, const float* __restrict__ weights, int n_tok,
+                               int K, int pieces, int wpt, typename Piece<BYTES>::type* __restrict__ drows,
+                               float* __restrict__ dweights) {
+  using P = typename Piece<BYTES>::type;
+  constexpr int W = BYTES / (int)sizeof(T), R = 8;
+  chain_wait();
+  __shared__ float s_part[kThreads / 32][R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * (kThreads / 32 / wpt) + warp / wpt, sub = warp % wpt;
+  const bool live = t < n_tok;
+  const int M = n_tok * K, n_rows = DROWS ? offsets[E] : M;
+  for (int k0 = 0; k0 < K; k0 += R) {
+    int p[R];
+    float w[R], dot[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const bool slot = live && k0 + j < K;
+      p[j] = slot ? row_of(pos, (size_t)t * K + k0 + j, M) : -1;
+      w[j] = DROWS && slot ? weights[(size_t)t * K + k0 + j] : 0.f;
+      dot[j] = 0.f;
+    }
+    for (int c = sub * 32 + lane; live && c < pieces; c += 32 * wpt) {
+      Values<T, BYTES> d, q[R];
+      d.raw = dout[(size_t)t * pieces + c];
+      if constexpr (DW) {
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+          if (p[j] >= 0) q[j].raw = rows[(size_t)p[j] * pieces + c];
+      }
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        if (DROWS && k0 + j < K && t * K + k0 + j >= n_rows) drows[(size_t)(t * K + k0 + j) * pieces + c] = zero_piece<P>();
+        if (p[j] < 0) continue;
+        if constexpr (DW) {
+#pragma unroll
+          for (int i = 0; i < W; ++i) dot[j] = fmaf(to_f32(q[j].v[i]), to_f32(d.v[i]), dot[j]);
+        }
+        if constexpr (DROWS) {
+          Values<T, BYTES> o;
+#pragma unroll
+          for (int i = 0; i < W; ++i) o.v[i] = from_f32<T>(w[j] * to_f32(d.v[i]));
+          drows[(size_t)p[j] * pieces + c] = o.raw;
+        }
+      }
+    }
+    if constexpr (DW) {
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        for (int off = 16; off; off >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], off);
+      if (wpt == 1) {
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+          if (lane == j && live && k0 + j < K) dweights[(size_t)t * K + k0 + j] = dot[j];
+      } else {                                     // (the same in the whole block)
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+          if (lane == j) s_part[warp][j] = dot[j];
+        __syncthreads();
+        if (sub == 0 && lane < R && live && k0 + lane < K) {
+          float sum = 0.f;
+          for (int i = 0; i < wpt; ++i) sum += s_part[warp + i][lane];
+          dweights[(size_t)t * K + k0 + lane] = sum;
+        }
+        __syncthreads();
+      }
+    }
+  }
+}
+
+// Bytes of the widest piece that divides the row and every pointer.
+int piece_bytes(size_t row_bytes, std::initializer_list<const void*> ptrs) {
+  uintptr_t bits = (uintptr_t)row_bytes;
+  for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
+  return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+}
+int lanes_for(int pieces) {
+  int lanes = 1;
+  while (lanes < pieces && lanes < kThreads) lanes *= 2;
+  return lanes;
+}
+
+int check_rows(const char* who, int T, int D, int K, int dtype) {
+  BWMOE_REQUIRE(T > 0 && D > 0 && K > 0, BWMOE_ERR_BAD_SHAPE, "%s: T=%d D=%d K=%d", who, T, D, K);
+  BWMOE_REQUIRE(K <= 32, BWMOE_ERR_UNSUPPORTED, "%s: K=%d > 32 slots per token", who, K);
+  BWMOE_REQUIRE((long long)T * K < (1ll << 31), BWMOE_ERR_UNSUPPORTED, "%s: T*K too large", who);
+  BWMOE_REQUIRE(D <= (1 << 24), BWMOE_ERR_UNSUPPORTED, "%s: D=%d too large", who, D);
+  BWMOE_REQUIRE(dtype >= BWMOE_BF16 && dtype <= BWMOE_F32, BWMOE_ERR_UNSUPPORTED, "%s: unknown type %d", who, dtype);
+  return BWMOE_OK;
+}
+int check_align(const char* who, int dtype, std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    BWMOE_REQUIRE(reinterpret_cast<uintptr_t>(p) % dtype_bytes(dtype) == 0, BWMOE_ERR_BAD_ALIGN,
+                  "%s: a pointer is not aligned to its type", who);
+  return BWMOE_OK;
+}
+
+template <int BYTES>
+int run_permute(const void* x, const int32_t* pos, const int32_t* offsets, int E, int T, int K, size_t row_bytes,
+                void* rows, cudaStream_t st) {
+  using P = typename Piece<BYTES>::type;
+  const int pieces = (int)(row_bytes / BYTES), lanes = lanes_for(ceil_div(pieces, 2));
+  const dim3 grid((unsigned)ceil_div(T, kThreads / lanes), (unsigned)ceil_div(pieces, 2 * lanes));
+  BWMOE_REQUIRE(grid.y <= 65535, BWMOE_ERR_UNSUPPORTED, "permute_rows: rows of %zu bytes", row_bytes);
+  BWMOE_CUDA_OK(launch_chained(permute_rows_kernel<BYTES>, grid, dim3(kThreads), 0, st, static_cast<const P*>(x), pos, offsets,
+                               E, T, K, pieces, lanes, static_cast<P*>(rows)));
+  return BWMOE_OK;
+}
+
+template <class T, int BYTES>
+int run_unpermute(const void* rows, const int32_t* pos, const float* weights, int n_tok, int K, size_t row_bytes, void* out,
+                  cudaStream_t st) {
+  using P = typename Piece<BYTES>::type;
+  const int pieces = (int)(row_bytes / BYTES), lanes = lanes_for(pieces);
+  const dim3 grid((unsigned)ceil_div(n_tok, kThreads / lanes), (unsigned)ceil_div(pieces, lanes));
+  BWMOE_REQUIRE(grid.y <= 65535, BWMOE_ERR_UNSUPPORTED, "unpermute_rows: rows of %zu bytes", row_bytes);
+  auto kernel = weights ? unpermute_rows_kernel<T, BYTES, true> : unpermute_rows_kernel<T, BYTES, false>;
+  BWMOE_CUDA_OK(launch_chained(kernel, grid, dim3(kThreads), 0, st, static_cast<const P*>(rows), pos, weights, n_tok, K,
+                               pieces, lanes, static_cast<P*>(out)));
+  return BWMOE_OK;
+}
+
+template <class T, int BYTES>
+int run_unpermute_backward(const void* dout, const void* rows, const int32_t* pos, const int32_t* offsets, int E,
+                           const float* weights, int n_tok, int K, size_t row_bytes, void* drows, float* dweights,
+                           cudaStream_t st) {
+  using P = typename Piece<BYTES>::type;
+  const int pieces = (int)(row_bytes / BYTES);
+  // warps per token: more while the row feeds them and the batch leaves the chip's warp slots empty
+  int wpt = 1;
+  while (wpt < 8 && 32 * wpt < pieces && (long long)n_tok * wpt < 16ll * sm_count()) wpt *= 2;
+  const unsigned blocks = (unsigned)ceil_div(n_tok, kThreads / 32 / wpt);
+  auto kernel = drows && dweights ? unpermute_rows_backward_kernel<T, BYTES, true, true>
+                : drows           ? unpermute_rows_backward_kernel<T, BYTES, true, false>
+                                  : unpermute_rows_backward_kernel<T, BYTES, false, true>;
+  BWMOE_CUDA_OK(launch_chained(kernel, dim3(blocks), dim3(kThreads), 0, st, static_cast<const P*>(dout),
+                               static_cast<const P*>(rows), pos, offsets, E, weights, n_tok, K, pieces, wpt,
+                               static_cast<P*>(drows), dweights));
+  return BWMOE_OK;
+}
+
+// fn(type tag, piece tag) for the element type and the widest piece
+template <class F>
+int for_type_and_piece(int dtype, int bytes, F fn) {
+  auto by_piece = [&](auto tag) {
+    using T = typename decltype(tag)::type;
+    switch (bytes) {
+      case 16: return fn(tag, std::integral_constant<int, 16>{});
+      case 8: return fn(tag, std::integral_constant<int, 8>{});
+      case 4: return fn(tag, std::integral_constant<int, 4>{});
+      default: return fn(tag, std::integral_constant<int, sizeof(T)>{});     // an fp32 row is never split below 4 bytes
+    }
+  };
+  if (dtype == BWMOE_F32) return by_piece(TypeTag<float>{});
+  if (dtype == BWMOE_F16) return by_piece(TypeTag<__half>{});
+  return by_piece(TypeTag<__nv_bfloat16>{});
+}
+
+}  // namespace
+
+int launch_permute_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
+                        void* rows, cudaStream_t st) {
+  if (int rc = check_rows("permute_rows", T, D, K, dtype)) return rc;
+  BWMOE_REQUIRE(E > 0, BWMOE_ERR_BAD_SHAPE, "permute_rows: E=%d", E);
+  BWMOE_REQUIRE(x && pos && offsets && rows, BWMOE_ERR_NULL, "permute_rows: null pointer");
+  if (int rc = check_align("permute_rows", dtype, {x, rows})) return rc;
+  const size_t row_bytes = (size_t)D * dtype_bytes(dtype);
+  switch (piece_bytes(row_bytes, {x, rows})) {
+    case 16: return run_permute<16>(x, pos, offsets, E, T, K, row_bytes, rows, st);
+    case 8: return run_permute<8>(x, pos, offsets, E, T, K, row_bytes, rows, st);
+    case 4: return run_permute<4>(x, pos, offsets, E, T, K, row_bytes, rows, st);
+    default: return run_permute<2>(x, pos, offsets, E, T, K, row_bytes, rows, st);
+  }
+}
+
+int launch_unpermute_rows(const void* rows, const int32_t* pos, const float* weights, int T, int D, int K, int dtype, void* out,
+                          cudaStream_t st) {
+  if (int rc = check_rows("unpermute_rows", T, D, K, dtype)) return rc;
+  BWMOE_REQUIRE(rows && pos && out, BWMOE_ERR_NULL, "unpermute_rows: null pointer");
+  if (int rc = check_align("unpermute_rows", dtype, {rows, out})) return rc;
+  const size_t row_bytes = (size_t)D * dtype_bytes(dtype);
+  return for_type_and_piece(dtype, piece_bytes(row_bytes, {rows, out}), [&](auto type, auto bytes) {
+    return run_unpermute<typename decltype(type)::type, decltype(bytes)::value>(rows, pos, weights, T, K, row_bytes, out, st);
+  });
+}
+
+int launch_unpermute_rows_backward(const void* dout, const void* rows, const int32_t* pos, const int32_t* offsets,
+                                   const float* weights, int T, int D, int E, int K, int dtype, void* drows, float* dweights,
+                                   cudaStream_t st) {
+  if (int rc = check_rows("unpermute_rows_backward", T, D, K, dtype)) return rc;
+  BWMOE_REQUIRE(dout && pos && (drows || dweights), BWMOE_ERR_NULL, "unpermute_rows_backward: null pointer");
+  BWMOE_REQUIRE(!drows || (offsets && weights && E > 0), BWMOE_ERR_NULL,
+                "unpermute_rows_backward: the rows' gradient needs offsets and weights");
+  BWMOE_REQUIRE(!dweights || rows, BWMOE_ERR_NULL, "unpermute_rows_backward: the weights' gradient needs the rows");
+  if (int rc = check_align("unpermute_rows_backward", dtype, {dout, rows, drows})) return rc;
+  const size_t row_bytes = (size_t)D * dtype_bytes(dtype);
+  return for_type_and_piece(dtype, piece_bytes(row_bytes, {dout, rows, drows}), [&](auto type, auto bytes) {
+    return run_unpermute_backward<typename decltype(type)::type, decltype(bytes)::value>(dout, rows, pos, offsets, E, weights, T,
+                                                                                         K, row_bytes, drows, dweights, st);
+  });
+}
+
+}  // namespace bwmoe

@@ -1,0 +1,223 @@
+// Activations -> 8-bit integers, one scale per row:
+//   scale = fl32(max|x| / 127)      code = x / scale rounded to the nearest whole number, ties to even
+// The scale is rounded to fp32 once and the codes are exact for that scale: a product with the reciprocal may end on the
+// wrong side of a border n + 1/2, so quotients that come near one are decided by the sign of x - (n + 1/2) * scale, which
+// one fused multiply-add gives exactly.  A row of zeros has scale 0 and codes 0.  A row with an infinity or a NaN has no
+// representation in 8 bits: its scale is NaN and its codes are 0, so that every product of the row is NaN.
+//
+// Bound by memory: a row is read once - each thread keeps its pieces of 16 elements in registers between the maximum and
+// the codes - and written to all of the rows it is needed in (the K rows of its token, or one).  The conversion adds
+// 1.5 * 2^23 instead of converting (the low byte of the sum is the code): at 3 bytes per element the conversion unit
+// (16 results per cycle and SM) would be as busy as the memory.
+#include "common.cuh"
+
+namespace bwmoe {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kKept = 4;                       // pieces of a row that a thread keeps in registers
+constexpr float kTinyScale = 7.888609052210118e-31f;     // 2^-100: below it products with the scale may lose bits
+
+// |x| / scale, rounded exactly (ties to even); scale > 0
+__device__ int exact_code(float x, float scale) {
+  const float a = fabsf(x), f = floorf(fminf(__fdiv_rn(a, scale), 127.f));
+  // the sign of a - (f + 1/2) * scale; doubled where the scale's last bits are the smallest there are
+  const float r = scale >= kTinyScale ? fmaf(-(f + 0.5f), scale, a) : fmaf(-(2.f * f + 1.f), scale, 2.f * a);
+  int q = (int)f;
+  if (r > 0.f || (r == 0.f && (q & 1))) ++q;
+  q = min(q, 127);
+  return x < 0.f ? -q : q;
+}
+
+template <class T> struct Piece16;             // 16 elements
+template <> struct Piece16<float> {
+  float4 r[4];
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = reinterpret_cast<const float4*>(p)[i];
+  }
+  __device__ __forceinline__ void values(float (&f)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[4 * i] = r[i].x, f[4 * i + 1] = r[i].y, f[4 * i + 2] = r[i].z, f[4 * i + 3] = r[i].w;
+  }
+};
+template <class T2, class T> __device__ __forceinline__ float2 pair_to_f32(uint32_t w);
+template <> __device__ __forceinline__ float2 pair_to_f32<__half2, __half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <> __device__ __forceinline__ float2 pair_to_f32<__nv_bfloat162, __nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <class T2, class T> struct Piece16Half {
+  uint4 r[2];
+  __device__ __forceinline__ void load(const T* p) {
+    r[0] = reinterpret_cast<const uint4*>(p)[0], r[1] = reinterpret_cast<const uint4*>(p)[1];
+  }
+  __device__ __forceinline__ void values(float (&f)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = pair_to_f32<T2, T>(w[j]);
+        f[8 * i + 2 * j] = v.x, f[8 * i + 2 * j + 1] = v.y;
+      }
+    }
+  }
+};
+template <> struct Piece16<__half> : Piece16Half<__half2, __half> {};
+template <> struct Piece16<__nv_bfloat16> : Piece16Half<__nv_bfloat162, __nv_bfloat16> {};
+
+template <class T>
+__device__ __forceinline__ uint32_t piece_amax_bits(const Piece16<T>& p) {
+  float f[16];
+  p.values(f);
+  uint32_t m = 0;       // of the bit patterns: infinities and NaN are larger than every number
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(fabsf(f[i])));
+  return m;
+}
+
+// scale >= kTinyScale and finite
+template <class T>
+__device__ __forceinline__ uint4 piece_codes(const Piece16<T>& p, float scale, float inv) {
+  constexpr float kMagic = 12582912.f;          // 1.5 * 2^23: the sum's last bit is worth 1
+  float f[16];
+  p.values(f);
+  uint32_t b[16];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float t = f[i] * inv, m = t + kMagic;
+    far = fmaxf(far, fabsf(t - (m - kMagic)));
+    b[i] = __float_as_uint(m);
+  }
+  // t is off by at most 127 * 2^-23 = 1.6e-5 (two roundings); anything nearer to a border is decided exactly
+  if (far > 0.4999f) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j == i) b[j] = (uint32_t)exact_code(f[j], scale);
+    }
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// wpr warps (1, 2, 4 or 8) share a row.  pos == nullptr: row t is written to row t.
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+quant_int8_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ pos, const int32_t* __restrict__ offsets, int E,
+                       int n_tok, int K, int D, int wpr, int8_t* __restrict__ codes, float* __restrict__ scales,
+                       uint32_t* __restrict__ zero, int zero_words) {
+  chain_wait();
+  __shared__ uint32_t s_max[kThreads / 32];
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < zero_words; i += kThreads) zero[i] = 0u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * (kThreads / 32 / wpr) + warp / wpr, sub = warp % wpr;
+  const bool live = t < n_tok;
+  const int pieces = D / 16, step = 32 * wpr, c0 = sub * 32 + lane;
+  const T* src = x + (size_t)t * D;
+  Piece16<T> kept[kKept];
+  uint32_t m = 0;
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < kKept; ++i)
+      if (c0 + i * step < pieces) kept[i].load(src + (size_t)(c0 + i * step) * 16);
+#pragma unroll
+    for (int i = 0; i < kKept; ++i)
+      if (c0 + i * step < pieces) m = max(m, piece_amax_bits(kept[i]));
+    for (int c = c0 + kKept * step; c < pieces; c += step) {      // rows longer than the registers hold
+      Piece16<T> q;
+      q.load(src + (size_t)c * 16);
+      m = max(m, piece_amax_bits(q));
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (wpr > 1) {                                // (the same in the whole block)
+    if (lane == 0) s_max[warp] = m;
+    __syncthreads();
+    for (int i = 0; i < wpr; ++i) m = max(m, s_max[warp - sub + i]);
+  }
+  if (!live) return;
+  const bool finite = m < 0x7f800000u;
+  const float scale = finite ? __fdiv_rn(__uint_as_float(m), 127.f) : __uint_as_float(0x7fc00000u);
+  const float inv = __fdiv_rn(1.f, scale);
+  auto convert = [&](const Piece16<T>& q) {
+    if (scale >= kTinyScale) return piece_codes(q, scale, inv);
+    uint4 o = make_uint4(0u, 0u, 0u, 0u);       // zeros, and rows that have no representation
+    if (finite && scale > 0.f) {
+      float f[16];
+      q.values(f);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[i] |= ((uint32_t)exact_code(f[4 * i + j], scale) & 0xffu) << (8 * j);
+      }
+      o = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return o;
+  };
+  const int M = n_tok * K, n_rows = pos != nullptr ? offsets[E] : M;
+  auto store = [&](int c, uint4 o) {
+    if (pos == nullptr) {
+      reinterpret_cast<uint4*>(codes + (size_t)t * D)[c] = o;
+      if (c == 0) scales[t] = scale;
+      return;
+    }
+#pragma unroll 4
+    for (int k = 0; k < K; ++k) {
+      const int s = t * K + k, p = pos[s];
+      if ((unsigned)p < (unsigned)M) {          // a plan is data from outside the kernel
+        reinterpret_cast<uint4*>(codes + (size_t)p * D)[c] = o;
+        if (c == 0) scales[p] = scale;
+      }
+      if (s >= n_rows) {                        // a row that no slot owns
+        reinterpret_cast<uint4*>(codes + (size_t)s * D)[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (c == 0) scales[s] = 0.f;
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (c0 + i * step < pieces) store(c0 + i * step, convert(kept[i]));
+  for (int c = c0 + kKept * step; c < pieces; c += step) {
+    Piece16<T> q;
+    q.load(src + (size_t)c * 16);
+    store(c, convert(q));
+  }
+}
+
+}  // namespace
+
+int launch_quant_int8_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
+                           void* codes, float* scales, cudaStream_t st, void* zero, size_t zero_bytes) {
+  BWMOE_REQUIRE(T > 0 && D > 0 && K > 0 && D % 16 == 0, BWMOE_ERR_BAD_SHAPE, "int_quant: T=%d D=%d K=%d (D a multiple of 16)", T, D, K);
+  BWMOE_REQUIRE((long long)T * K < (1ll << 31), BWMOE_ERR_UNSUPPORTED, "int_quant: T*K too large");
+  BWMOE_REQUIRE(dtype >= BWMOE_BF16 && dtype <= BWMOE_F32, BWMOE_ERR_UNSUPPORTED, "int_quant: unknown type %d", dtype);
+  BWMOE_REQUIRE(x && codes && scales, BWMOE_ERR_NULL, "int_quant: null pointer");
+  BWMOE_REQUIRE(pos == nullptr ? K == 1 : (offsets != nullptr && E > 0), BWMOE_ERR_BAD_SHAPE,
+                "int_quant: K=%d needs the slots' places and the segments' offsets", K);
+  BWMOE_REQUIRE(aligned16(x) && aligned16(codes) && reinterpret_cast<uintptr_t>(scales) % 4 == 0, BWMOE_ERR_BAD_ALIGN,
+                "int_quant: x and codes must be 16-byte aligned");
+  const int pieces = D / 16;
+  int wpr = 1;      // warps per row: until the row fits the registers, and more while the batch leaves the chip empty
+  while (wpr < 8 && 32 * wpr < pieces && (32 * wpr * kKept < pieces || (long long)T * wpr < 32ll * sm_count())) wpr *= 2;
+  const dim3 grid((unsigned)ceil_div(T, kThreads / 32 / wpr));
+  auto run = [&](auto tag) {
+    using X = typename decltype(tag)::type;
+    return launch_chained(quant_int8_rows_kernel<X>, grid, dim3(kThreads), 0, st, static_cast<const X*>(x), pos, offsets, E, T, K,
+                          D, wpr, static_cast<int8_t*>(codes), scales, static_cast<uint32_t*>(zero), (int)(zero_bytes / 4));
+  };
+  BWMOE_CUDA_OK(dtype == BWMOE_F32 ? run(TypeTag<float>{}) : dtype == BWMOE_F16 ? run(TypeTag<__half>{}) : run(TypeTag<__nv_bfloat16>{}));
+  return BWMOE_OK;
+}
+
+}  // namespace bwmoe

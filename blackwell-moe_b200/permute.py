@@ -1,0 +1,236 @@
+"""Tokens into expert order and back, with gradients.
+
+The permutation of the MoE block as operators of their own, for programs that run their own computation between the two
+- experts in another format, an adapter, a training step: ``permute_tokens`` takes over ``permute_tokens``
+(src/blackwell_moe/kernels/permute.py:12-39), ``unpermute_tokens`` takes over ``unpermute_and_combine``
+(src/blackwell_moe/kernels/permute.py:42-59).  bf16, fp16 and fp32; sums are held in fp32, added in a fixed order and
+rounded once.  Both are differentiable (once): in the tokens and the rows, and in the routing weights.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .moe import _contig, _require_cuda, _stream
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+class PermutePlan(NamedTuple):
+    """Where every slot (token, k) of a batch goes in expert order; int32 tensors of one device.
+
+    ``offsets[E+1]``: expert e's rows are ``offsets[e] .. offsets[e+1]-1``; ``pos[T,K]``: the row of each slot;
+    ``row_slot[M]``: the slot of each row, ``t*K + k``; ``row_expert[M]``: its expert.  A slot whose expert id is
+    outside ``[0, E)`` has no row (``pos`` -1), and the rows past ``offsets[E]`` then have no slot (-1)."""
+    offsets: torch.Tensor
+    pos: torch.Tensor
+    row_slot: torch.Tensor
+    row_expert: torch.Tensor
+
+
+def _dtype_code(t: torch.Tensor, name: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: {t.dtype} is not one of bfloat16, float16, float32")
+    return code
+
+
+def _empty_plan(T, K, num_experts, dev):
+    M = T * K
+    o, p, s, e = torch.empty(num_experts + 1 + 3 * M, dtype=torch.int32, device=dev).split((num_experts + 1, M, M, M))
+    return PermutePlan(o, p.view(T, K), s, e)
+
+
+def _check_indices(indices, num_experts):
+    assert indices.dim() == 2 and indices.shape[1] >= 1, indices.shape
+    assert indices.dtype == torch.int32, indices.dtype
+    if not 1 <= num_experts <= 256 or indices.shape[1] > 32:
+        raise ValueError(f"{num_experts} experts and {indices.shape[1]} slots per token: at most 256 and 32")
+    return _contig(indices, "indices")
+
+
+def _check_plan(plan, name="plan"):
+    offsets, pos = plan[0], plan[1]
+    assert pos.dim() == 2 and offsets.dim() == 1 and offsets.numel() >= 2, (name, pos.shape, offsets.shape)
+    assert pos.dtype == torch.int32 and offsets.dtype == torch.int32, (name, pos.dtype, offsets.dtype)
+    _contig(pos, "plan.pos"), _contig(offsets, "plan.offsets")
+    return offsets, pos
+
+
+def _plan_scratch(lib, T, E, K, dev):
+    # the plan's scratch, and a status word behind it
+    n = lib.bwmoe_plan_scratch_bytes(T, E, K)
+    ws = torch.empty(n + 16, dtype=torch.uint8, device=dev)
+    return ws, n
+
+
+def permute_plan(indices: torch.Tensor, num_experts: int) -> PermutePlan:
+    """The stable sort of all slots of ``indices[T,K]`` int32 by expert id."""
+    indices = _check_indices(indices, num_experts)
+    dev = _require_cuda(indices)
+    T, K = indices.shape
+    with torch.cuda.device(dev):
+        plan = _empty_plan(T, K, num_experts, dev)
+        if T == 0:
+            plan.offsets.zero_()
+            return plan
+        lib = _lib.lib()
+        ws, n = _plan_scratch(lib, T, num_experts, K, dev)
+        _lib.check(lib.bwmoe_permute_plan(indices.data_ptr(), None, T, num_experts, K, *[t.data_ptr() for t in plan], None,
+                                          ws.data_ptr() + n, ws.data_ptr(), _stream(dev)))
+    return plan
+
+
+def _permute(x, plan):
+    """rows[pos[t,k]] = x[t]"""
+    T, K = plan.pos.shape
+    rows = torch.empty((T * K, x.shape[1]), dtype=x.dtype, device=x.device)
+    if rows.numel():
+        with torch.cuda.device(x.device):
+            _lib.check(_lib.lib().bwmoe_permute_rows(x.data_ptr(), plan.pos.data_ptr(), plan.offsets.data_ptr(), T, x.shape[1],
+                                                     plan.offsets.numel() - 1, K, _DTYPES[x.dtype], rows.data_ptr(),
+                                                     _stream(x.device)))
+    return rows
+
+
+def _unpermute(rows, pos, weights):
+    """sum over k of w[t,k] * rows[pos[t,k]]"""
+    T, K = pos.shape
+    out = torch.empty((T, rows.shape[1]), dtype=rows.dtype, device=rows.device)
+    if out.numel():
+        with torch.cuda.device(rows.device):
+            _lib.check(_lib.lib().bwmoe_unpermute_rows(rows.data_ptr(), pos.data_ptr(),
+                                                       None if weights is None else weights.data_ptr(), T, rows.shape[1], K,
+                                                       _DTYPES[rows.dtype], out.data_ptr(), _stream(rows.device)))
+    return out
+
+
+class _PermuteRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, offsets, pos):
+        ctx.save_for_backward(pos)
+        return _permute(x, PermutePlan(offsets, pos, None, None))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, drows):
+        return _unpermute(drows.contiguous(), ctx.saved_tensors[0], None), None, None
+
+
+class _PermuteTokens(torch.autograd.Function):
+    """The plan and the rows in one call."""
+
+    @staticmethod
+    def forward(ctx, x, indices, num_experts):
+        T, K = indices.shape
+        D, dev = x.shape[1], x.device
+        plan = _empty_plan(T, K, num_experts, dev)
+        rows = torch.empty((T * K, D), dtype=x.dtype, device=dev)
+        lib = _lib.lib()
+        with torch.cuda.device(dev):
+            ws, n = _plan_scratch(lib, T, num_experts, K, dev)
+            _lib.check(lib.bwmoe_permute_tokens(x.data_ptr(), indices.data_ptr(), T, D, num_experts, K, _DTYPES[x.dtype],
+                                                *[t.data_ptr() for t in plan], rows.data_ptr(), ws.data_ptr() + n,
+                                                ws.data_ptr(), _stream(dev)))
+        ctx.save_for_backward(plan.pos)
+        ctx.mark_non_differentiable(*plan)
+        return (rows, *plan)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, drows, *_):
+        return _unpermute(drows.contiguous(), ctx.saved_tensors[0], None), None, None
+
+
+class _UnpermuteRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, offsets, pos, weights):
+        # the rows are kept for the weights' gradient only
+        ctx.save_for_backward(rows if ctx.needs_input_grad[3] else None, offsets, pos, weights)
+        return _unpermute(rows, pos, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        rows, offsets, pos, weights = ctx.saved_tensors
+        dout = dout.contiguous()
+        if weights is None:
+            return _permute(dout, PermutePlan(offsets, pos, None, None)), None, None, None
+        drows, dweights = unpermute_tokens_backward(dout, rows, PermutePlan(offsets, pos, None, None), weights,
+                                                    rows_grad=ctx.needs_input_grad[0], weights_grad=ctx.needs_input_grad[3])
+        return drows, None, None, dweights
+
+
+def permute_tokens(x: torch.Tensor, indices: torch.Tensor = None, num_experts: int = None, *, plan: PermutePlan = None):
+    """``x[T,D]`` -> ``(rows[T*K,D], plan)``: a copy of token t in the row of each of its slots, rows sorted by expert
+    (stable).  ``indices[T,K]`` int32 are the tokens' experts; or pass the ``plan`` of an earlier call.  Rows that no slot
+    owns are zero.  The gradient of a token is the sum of its rows' gradients."""
+    assert x.dim() == 2, x.shape
+    code = _dtype_code(x, "x")
+    x = _contig(x, "x")
+    if (indices is None) == (plan is None) or (indices is None) != (num_experts is None):
+        raise ValueError("permute_tokens takes indices and num_experts, or a plan")
+    if plan is not None:
+        offsets, pos = _check_plan(plan)
+        assert pos.shape[0] == x.shape[0], (pos.shape, x.shape)
+        _require_cuda(x, offsets, pos)
+        return _PermuteRows.apply(x, offsets, pos), plan
+    indices = _check_indices(indices, num_experts)
+    assert indices.shape[0] == x.shape[0], (indices.shape, x.shape)
+    _require_cuda(x, indices)
+    if x.numel() == 0:
+        plan = permute_plan(indices, num_experts)
+        return _PermuteRows.apply(x, plan.offsets, plan.pos), plan
+    rows, *parts = _PermuteTokens.apply(x, indices, num_experts)
+    return rows, PermutePlan(*parts)
+
+
+def _check_unpermute(rows, plan, weights):
+    assert rows.dim() == 2, rows.shape
+    _dtype_code(rows, "rows")
+    offsets, pos = _check_plan(plan)
+    assert rows.shape[0] == pos.numel(), (rows.shape, pos.shape)
+    tensors = [_contig(rows, "rows"), offsets, pos]
+    if weights is not None:
+        assert weights.shape == pos.shape and weights.dtype == torch.float32, (weights.shape, weights.dtype)
+        tensors.append(_contig(weights, "weights"))
+    _require_cuda(*tensors)
+    return offsets, pos
+
+
+def unpermute_tokens(rows: torch.Tensor, plan: PermutePlan, weights: torch.Tensor = None) -> torch.Tensor:
+    """``rows[T*K,D]`` in expert order -> ``out[T,D]``, ``out[t] = sum_k weights[t,k] * rows[plan.pos[t,k]]`` with
+    ``weights[T,K]`` fp32 (absent: 1).  Slots without a row add nothing.  Differentiable in ``rows`` and ``weights``."""
+    offsets, pos = _check_unpermute(rows, plan, weights)
+    return _UnpermuteRows.apply(rows, offsets, pos, weights)
+
+
+def unpermute_tokens_backward(dout: torch.Tensor, rows: torch.Tensor, plan: PermutePlan, weights: torch.Tensor, *,
+                              rows_grad: bool = True, weights_grad: bool = True):
+    """The gradients of :func:`unpermute_tokens` without autograd, for programs that run (or capture) their backward pass
+    themselves: ``(drows, dweights)``, ``None`` where not asked for.  ``rows`` may be ``None`` without ``weights_grad``."""
+    assert dout.dim() == 2, dout.shape
+    code = _dtype_code(dout, "dout")
+    offsets, pos = _check_plan(plan)
+    (T, K), D, dev = pos.shape, dout.shape[1], dout.device
+    assert dout.shape[0] == T, (dout.shape, pos.shape)
+    assert weights.shape == pos.shape and weights.dtype == torch.float32, (weights.shape, weights.dtype)
+    tensors = [_contig(dout, "dout"), offsets, pos, _contig(weights, "weights")]
+    if weights_grad:
+        assert rows is not None and rows.shape == (T * K, D) and rows.dtype == dout.dtype, (None if rows is None else rows.shape)
+        tensors.append(_contig(rows, "rows"))
+    _require_cuda(*tensors)
+    drows = torch.empty((T * K, D), dtype=dout.dtype, device=dev) if rows_grad else None
+    dweights = torch.empty((T, K), dtype=torch.float32, device=dev) if weights_grad else None
+    if T == 0 or D == 0:
+        return drows, (dweights.zero_() if weights_grad else None)
+    if rows_grad or weights_grad:
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().bwmoe_unpermute_rows_backward(
+                dout.data_ptr(), rows.data_ptr() if weights_grad else None, pos.data_ptr(), offsets.data_ptr(),
+                weights.data_ptr(), T, D, offsets.numel() - 1, K, code, drows.data_ptr() if rows_grad else None,
+                dweights.data_ptr() if weights_grad else None, _stream(dev)))
+    return drows, dweights

@@ -54,3 +54,19 @@ def quantize_expert_weights_block(w: torch.Tensor):
     """:func:`quant_fp8_block_128` over a stack ``[E, in, out]`` -> ``(codes, scale_inv[E, in/128, out/128])``."""
     qs, ss = zip(*(quant_fp8_block_128(w[e]) for e in range(w.shape[0])))
     return torch.stack(list(qs)).contiguous(), torch.stack(list(ss)).contiguous()
+
+
+def quant_int8_channels(w: torch.Tensor):
+    """8-bit integers with one scale for each output channel of ``w[..., in, out]``: ``(codes int8, scales[..., out] fp32)``
+    with ``codes * scales ~= w``; codes in [-127, 127], a channel of zeros has scale 0."""
+    wf = w.to(torch.float32)
+    amax = wf.abs().amax(dim=-2)
+    scales = amax / torch.full_like(amax, 127.0)       # tensor / tensor: an IEEE division on every device
+    safe = torch.where(scales > 0, scales, torch.ones_like(scales))
+    return torch.round(wf / safe.unsqueeze(-2)).clamp_(-127, 127).to(torch.int8), scales
+
+
+def quantize_expert_weights_int8(w: torch.Tensor):
+    """:func:`quant_int8_channels` over a stack ``[E, in, out]``, expert by expert -> ``(codes, scales[E, out])``."""
+    qs, ss = zip(*(quant_int8_channels(w[e]) for e in range(w.shape[0])))
+    return torch.stack(list(qs)).contiguous(), torch.stack(list(ss)).contiguous()

@@ -54,6 +54,13 @@ enum {
                                     the surplus rows were dropped, not written past the buffer */
 };
 
+/* Element types of the entry points that take more than one (permutation, 8-bit integers). */
+enum {
+  BWMOE_BF16 = 0,
+  BWMOE_F16 = 1,
+  BWMOE_F32 = 2
+};
+
 /* Selectors for bwmoe_workspace_view: intermediates kept in the workspace after
  * a forward, exposed so that tests can check each stage bit for bit. */
 enum {
@@ -488,6 +495,81 @@ int bwmoe_scatter_quant_peers(const void* d_x, const int32_t* d_pos, const int32
 int bwmoe_combine_peers(void* const* h_y_of_rank, int n_ranks, const int32_t* d_pos, const int32_t* d_indices,
                         const float* d_weights, const int32_t* d_delta, int experts_per_rank, int T, int D,
                         int K, void* d_out, void* stream);
+
+/*
+ * ---- tokens into expert order and back, in bf16, fp16 or fp32 (dtype: BWMOE_BF16 ...), with gradients ----
+ *
+ * M = T*K rows; d_pos[T,K] and d_offsets[E+1] as bwmoe_permute_plan writes them.  Sums are held in fp32 and rounded once;
+ * results are the same on every call.  Any D; K <= 32.  Pointers are aligned to their type (rows of a multiple of 16 bytes
+ * at 16-byte aligned addresses move fastest).  A place outside [0, M) is no row: its slot adds nothing, and its weight's gradient is
+ * 0.  The rows d_offsets[E] .. M-1, which no slot owns (expert ids out of range), are written as zeros.
+ *
+ * bwmoe_permute_tokens: bwmoe_permute_plan, then bwmoe_permute_rows.  Scratch: bwmoe_plan_scratch_bytes(T, E, K).
+ * replaces: permute_tokens, src/blackwell_moe/kernels/permute.py:12-39.
+ */
+int bwmoe_permute_tokens(const void* d_x, const int32_t* d_indices, int T, int D, int E, int K, int dtype,
+                         int32_t* d_offsets, int32_t* d_pos, int32_t* d_row_slot, int32_t* d_row_expert,
+                         void* d_rows, int32_t* d_status, void* d_scratch, void* stream);
+/* d_rows[pos[t,k],:] = x[t,:].  No counterpart of its own in the reference (a gather inside permute_tokens). */
+int bwmoe_permute_rows(const void* d_x, const int32_t* d_pos, const int32_t* d_offsets, int T, int D, int E, int K,
+                       int dtype, void* d_rows, void* stream);
+/* out[t,:] = sum_k w[t,k] * rows[pos[t,k],:], k ascending, d_weights[T,K] fp32; null: weights of 1 (which is the gradient
+ * of bwmoe_permute_rows).
+ * replaces: unpermute_and_combine, src/blackwell_moe/kernels/permute.py:42-59. */
+int bwmoe_unpermute_rows(const void* d_rows, const int32_t* d_pos, const float* d_weights, int T, int D, int K, int dtype,
+                         void* d_out, void* stream);
+/* Gradients of bwmoe_unpermute_rows: d_drows[pos[t,k],:] = w[t,k] * dout[t,:] and d_dweights[t,k] = <rows[pos[t,k],:],
+ * dout[t,:]> (fp32).  Either may be null; d_rows is needed for the second, weights and offsets for the first.
+ * No counterpart in the reference (inference only). */
+int bwmoe_unpermute_rows_backward(const void* d_dout, const void* d_rows, const int32_t* d_pos, const int32_t* d_offsets,
+                                  const float* d_weights, int T, int D, int E, int K, int dtype, void* d_drows,
+                                  float* d_dweights, void* stream);
+
+/*
+ * ---- experts in 8-bit integers ("int"): a scale for each row of the activations and for each channel of the weights ----
+ *
+ * value = code * scale on both sides.  Weights [E, K, N] int8, N contiguous, channel scales [E, N] fp32.  Products are
+ * summed in 32-bit integers (exact; K < 131072), scaled in fp32 and rounded once to the output type.  K and N are
+ * multiples of 16, E <= 256.  No counterpart in the reference (its integer path is 4-bit, weights only).
+ *
+ * bwmoe_int_quant: scale[t] = fl32(max|x[t,:]| / 127), codes = x / scale rounded to nearest, ties to even, exactly.  A
+ * row of zeros gets scale 0; a row with an infinity or a NaN gets scale NaN and codes 0, which makes its products NaN.
+ * With d_pos (and d_offsets) codes and scale go to the token's K rows in expert order, [T*K, D] and [T*K] (rows that no
+ * slot owns: zeros); d_pos null, K = 1: in place of the token.
+ */
+int bwmoe_int_quant(const void* d_x, const int32_t* d_pos, const int32_t* d_offsets, int T, int D, int E, int K, int dtype,
+                     void* d_codes, float* d_scales, void* stream);
+/* out[m,:] = (codes[m,:] x w[e]) * row_scale[m] * channel_scale[e,:] for the rows m of segment e; d_offsets null with E = 1:
+ * every row.  Rows behind the last segment are written as zeros.  dtype: of the result.
+ * d_scratch: bwmoe_int_scratch_bytes() bytes, 16-byte aligned; its first word is the call's status word (BWMOE_STATUS_*). */
+size_t bwmoe_int_scratch_bytes(int M, int K, int N, int E);
+int bwmoe_int_grouped_gemm(const void* d_codes, const float* d_row_scale, const int32_t* d_offsets, const void* d_w,
+                            const float* d_scale, int M, int K, int N, int E, int dtype, void* d_out, void* d_scratch,
+                            size_t scratch_bytes, void* stream);
+/* h = silu(codes x w_gate) * (codes x w_up), scaled as above; d_scratch as above. */
+int bwmoe_int_gateup_swiglu(const void* d_codes, const float* d_row_scale, const int32_t* d_offsets, const void* d_w_gate,
+                             const void* d_w_up, const float* d_scale_gate, const float* d_scale_up, int M, int K, int N,
+                             int E, int dtype, void* d_h, void* d_scratch, size_t scratch_bytes, void* stream);
+/* bwmoe_int_quant and the product of all rows with one matrix [K,N]; dtype: of x and of the result. */
+size_t bwmoe_workspace_bytes_int_matmul(int T, int K, int N);
+int bwmoe_int_matmul(const void* d_x, const void* d_w, const float* d_scale, int T, int K, int N, int dtype, void* d_out,
+                      void* d_workspace, size_t workspace_bytes, void* stream);
+/*
+ * The block over experts in 8-bit integers: quantise -> gate/up -> SwiGLU (h in x's type) -> quantise h row by row -> down (in x's
+ * type) -> sum with the routing weights.  dtype: BWMOE_BF16 or BWMOE_F16, of x and out; weights [E,D,H], [E,D,H], [E,H,D],
+ * scales [E,H], [E,H], [E,D].  bwmoe_moe_forward_int routes with bwmoe_router (bf16 only).  The status word is the
+ * workspace's first (bwmoe_read_status); an expert id out of range contributes nothing and raises BWMOE_STATUS_BAD_EXPERT.
+ */
+size_t bwmoe_workspace_bytes_int(int T, int D, int H, int E, int K);
+int bwmoe_moe_forward_int_routed(const void* d_x, const float* d_weights, const int32_t* d_indices,
+                                  const void* d_experts_w_gate, const void* d_experts_w_up, const void* d_experts_w_down,
+                                  const float* d_scales_gate, const float* d_scales_up, const float* d_scales_down,
+                                  int T, int D, int H, int E, int K, int dtype, void* d_out, void* d_workspace,
+                                  size_t workspace_bytes, void* stream);
+int bwmoe_moe_forward_int(const void* d_x, const void* d_w_gate, const void* d_experts_w_gate,
+                           const void* d_experts_w_up, const void* d_experts_w_down, const float* d_scales_gate,
+                           const float* d_scales_up, const float* d_scales_down, int T, int D, int H, int E, int K,
+                           void* d_out, void* d_workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

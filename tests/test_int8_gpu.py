@@ -1,0 +1,309 @@
+"""Experts in 8-bit integers: the row quantiser, the grouped products and the block, against the definitions in 64 bits."""
+
+import pytest
+import torch
+
+import blackwell_moe_b200 as bw
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F16, F32, I8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
+U32 = 2.0 ** -24                                 # half a step of fp32
+
+
+def half_step(dtype):
+    return 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+
+
+def smallest_step(dtype):
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+def exact_codes(x):
+    """Codes and scales by the definition; the quotients in 64 bits are exact enough to tell a tie from its neighbours
+    (they differ from n + 1/2 by 2^-33 at least, or not at all).  A row with an infinity or a NaN has none."""
+    x = x.double()
+    amax = x.abs().amax(1)
+    scale = (torch.where(amax.isfinite(), amax, torch.full_like(amax, float("nan"))) / 127).float().double()
+    q = torch.where(scale[:, None] > 0, x / scale[:, None], torch.zeros_like(x))
+    return torch.round(q).clamp(-127, 127).to(I8), scale.float()
+
+
+def assert_codes(codes, scales, x):
+    want, scale = exact_codes(x)
+    torch.testing.assert_close(scales.cpu(), scale, rtol=0, atol=0, equal_nan=True)
+    assert torch.equal(codes.cpu(), want), torch.nonzero(codes.cpu() != want)[:8].tolist()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,D", [(1, 16), (3, 48), (64, 2048), (517, 1408), (5, 14336), (2, 16384), (3, 20000), (6000, 64)])
+def test_codes_are_exact(T, D, dtype):
+    g = torch.Generator().manual_seed(T + D)
+    x = (torch.randn(T, D, generator=g) * torch.exp(3 * torch.randn(T, 1, generator=g))).to(dtype)
+    codes, scales = bw.quantize_tokens_int8(x.to(DEV))
+    assert_codes(codes, scales, x)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_codes_on_borders_and_of_small_rows(dtype):
+    D = 1024
+    n = torch.arange(D) % 255 - 127
+    ties = (n.float() + 0.5).clamp(-127, 127)
+    rows = [ties * 2.0 ** -4, ties * 2.0 ** -8, n.float(), torch.zeros(D)]     # the largest is 127 steps: the scale is exact
+    g = torch.Generator().manual_seed(3)
+    tiny = torch.finfo(dtype).smallest_normal
+    rows += [torch.randn(D, generator=g) * s for s in (tiny, tiny * 2 ** -4, tiny * 2 ** -6, tiny * 2 ** -7, tiny * 200)]
+    rows += [torch.randn(D, generator=g).clamp(-1, 1) * torch.finfo(dtype).max * 0.99]
+    one = torch.zeros(D)
+    one[700] = -smallest_step(dtype)
+    rows += [one, -0.0 * one]
+    x = torch.stack(rows).to(dtype)
+    if dtype != F32:
+        x[0, 0] = 127 * 2.0 ** -4
+    # fp32: values next to the borders of a scale that is not a power of two
+    s = torch.tensor(0.0123).float()
+    near = ((torch.arange(D) % 127).double() + 0.5) * s.double()
+    near = near.float() if dtype == F32 else near.to(dtype).float()
+    if dtype == F32:
+        near[1::3] = torch.nextafter(near[1::3], torch.tensor(9e9))
+        near[2::3] = torch.nextafter(near[2::3], torch.tensor(-9e9))
+    near[5] = 127 * s
+    x = torch.cat([x, near[None].to(dtype), -near[None].to(dtype)])
+    codes, scales = bw.quantize_tokens_int8(x.to(DEV))
+    assert_codes(codes, scales, x)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_rows_without_a_representation(dtype):
+    x = torch.ones(6, 64, dtype=dtype)
+    x[1, 3], x[2, 63], x[3, 0] = float("nan"), float("inf"), -float("inf")
+    codes, scales = bw.quantize_tokens_int8(x.to(DEV))
+    assert scales.isnan().tolist() == [False, True, True, True, False, False]
+    assert (codes[1:4] == 0).all() and (codes[0] == 127).all() and (codes[4:] == 127).all()
+    w = torch.ones(64, 32, dtype=I8, device=DEV)
+    out = bw.int8_matmul(x.to(DEV), w, torch.ones(32, device=DEV))
+    assert out.isnan().any(1).tolist() == out.isnan().all(1).tolist() == [False, True, True, True, False, False]
+
+
+@pytest.mark.parametrize("T,D,E,K,bad", [(1, 16, 4, 2, 0), (37, 2048, 64, 6, 5), (700, 144, 16, 3, 11)])
+def test_codes_in_expert_order(T, D, E, K, bad):
+    g = torch.Generator().manual_seed(T)
+    idx = torch.rand(T, E, generator=g).topk(K, 1).indices.to(torch.int32)
+    idx.view(-1)[torch.randperm(T * K, generator=g)[:bad]] = E
+    x = torch.randn(T, D, generator=g).to(BF16).to(DEV)
+    plan = bw.permute_plan(idx.to(DEV), E)
+    codes, scales = bw.quantize_tokens_int8(x, plan)
+    alone, s = bw.quantize_tokens_int8(x)
+    n = T * K - bad
+    tok = plan.row_slot[:n].long() // K
+    assert torch.equal(codes[:n], alone[tok]) and torch.equal(scales[:n], s[tok])
+    assert (codes[n:] == 0).all() and (scales[n:] == 0).all()
+
+
+def make_segments(counts, M):
+    return torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32), M - sum(counts)
+
+
+def make_codes(shape, seed, extreme=False):
+    g = torch.Generator().manual_seed(seed)
+    if extreme:
+        return torch.full(shape, -128, dtype=I8)
+    return torch.randint(-128, 128, shape, generator=g, dtype=torch.int16).to(I8)
+
+
+# rows of each expert, rows without one, K, N
+GROUPED = [([1], 0, 16, 16), ([3], 0, 4096, 512), ([0, 2, 0, 1], 2, 48, 32), ([130, 0, 5], 0, 144, 272), ([128, 256, 17], 40, 384, 1040),
+           ([1, 300, 7, 0, 90], 3, 1408, 528), ([0, 0], 4, 64, 64), ([2] * 64, 0, 2048, 1408), ([33, 1, 64, 65, 31], 0, 2064, 256),
+           ([600], 0, 512, 4112), ([0] * 255 + [9], 1, 128, 128), ([700] * 3, 0, 256, 768)]
+
+
+@pytest.mark.parametrize("counts,loose,K,N", GROUPED)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_grouped_product(counts, loose, K, N, dtype):
+    M, E = sum(counts) + loose, len(counts)
+    offsets, _ = make_segments(counts, M)
+    a, w = make_codes((M, K), 1), make_codes((E, K, N), 2)
+    g = torch.Generator().manual_seed(3)
+    rs = torch.rand(M, generator=g) * 1e-2
+    cs = torch.rand(E, N, generator=g) * 1e-3
+    out = bw.int8_grouped_gemm(a.to(DEV), rs.to(DEV), offsets.to(DEV), w.to(DEV), cs.to(DEV), out_dtype=dtype).cpu()
+    assert out.dtype == dtype and out.shape == (M, N)
+    n = sum(counts)
+    expert = torch.repeat_interleave(torch.arange(E), torch.tensor(counts))
+    for e in range(E):
+        rows = torch.nonzero(expert == e).flatten()
+        if len(rows):
+            acc = (a[rows].to(DEV).double() @ w[e].to(DEV).double()).cpu()             # whole numbers below 2^53: exact
+            ref = acc * rs[rows, None].double() * cs[e].double()
+            # the sum's conversion and two products, then the rounding to the type
+            bound = ref.abs() * (3.01 * U32 + half_step(dtype) * 1.001) + smallest_step(dtype)
+            assert ((out[rows].double() - ref).abs() <= bound).all(), e
+    assert (out[n:] == 0).all()
+
+
+def swiglu_bound(g, u, dtype):
+    """silu(g) * u in fp32 from a gate and an up product that are 3 roundings off: the gate's error counts (1 + |g|) times in
+    silu; the exponential is off by (2 + 1.16 |g|) steps, the quotient by 2, four more roundings."""
+    ref = g * torch.sigmoid(g) * u
+    rel = (3 * (1 + g.abs()) + 3 + 2 * (2 + 1.16 * g.abs()) + 4 + 4) * U32
+    # below exp(-87) the quotient of the fast form is 0 instead of a number below 2^-118
+    return ref, ref.abs() * (rel * 1.01 + half_step(dtype) * 1.001) + smallest_step(dtype) + u.abs() * 2.0 ** -118
+
+
+@pytest.mark.parametrize("counts,loose,K,N", GROUPED)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_grouped_swiglu(counts, loose, K, N, dtype):
+    M, E = sum(counts) + loose, len(counts)
+    offsets, _ = make_segments(counts, M)
+    a, wg, wu = make_codes((M, K), 1), make_codes((E, K, N), 2), make_codes((E, K, N), 5)
+    g = torch.Generator().manual_seed(3)
+    rs = torch.rand(M, generator=g) * 1e-2
+    sg, su = (torch.rand(E, N, generator=g) * 2e-2 / K ** 0.5 for _ in range(2))
+    sg[:, ::7] *= 20                                # gates far on either side
+    out = bw.int8_grouped_swiglu(a.to(DEV), rs.to(DEV), offsets.to(DEV), wg.to(DEV), wu.to(DEV), sg.to(DEV), su.to(DEV),
+                                 out_dtype=dtype).cpu()
+    expert = torch.repeat_interleave(torch.arange(E), torch.tensor(counts))
+    for e in range(E):
+        rows = torch.nonzero(expert == e).flatten()
+        if len(rows):
+            x = a[rows].to(DEV).double()
+            gate, up = (((x @ w[e].to(DEV).double()).cpu() * rs[rows, None].double() * s[e].double()) for w, s in ((wg, sg), (wu, su)))
+            ref, bound = swiglu_bound(gate, up, dtype)
+            assert ((out[rows].double() - ref).abs() <= bound).all(), e
+    assert (out[sum(counts):] == 0).all()
+
+
+@pytest.mark.parametrize("K", [16, 2048, 131056])
+@pytest.mark.parametrize("M", [1, 200])
+def test_largest_sums(M, K):
+    """-128 * -128 everywhere: 2^14 K, which for the largest K is just below 2^31."""
+    a, w = make_codes((M, K), 0, True).to(DEV), make_codes((1, K, 32), 0, True).to(DEV)
+    offsets = torch.tensor([0, M], dtype=torch.int32, device=DEV)
+    out = bw.int8_grouped_gemm(a, torch.ones(M, device=DEV), offsets, w, torch.ones(1, 32, device=DEV), out_dtype=F32)
+    assert (out == float(2 ** 14 * K)).all()      # 2^18 times a 13-bit number: exact in fp32
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,K,N", [(1, 16, 16), (1, 4096, 1024), (7, 2064, 272), (64, 1408, 2064), (517, 1408, 2064), (1500, 256, 640)])
+def test_matmul(T, K, N, dtype):
+    g = torch.Generator().manual_seed(T + K)
+    x = torch.randn(T, K, generator=g).to(dtype)
+    w, s = bw.quant_int8_channels(torch.randn(K, N, generator=g) * 0.02)
+    out = bw.int8_matmul(x.to(DEV), w.to(DEV), s.to(DEV)).cpu()
+    codes, scale = exact_codes(x)
+    ref = (codes.to(DEV).double() @ w.to(DEV).double()).cpu() * scale[:, None].double() * s.double()
+    assert ((out.double() - ref).abs() <= ref.abs() * (3.01 * U32 + half_step(dtype) * 1.001) + smallest_step(dtype)).all()
+
+
+def make_block(T, D, H, E, K, dtype, seed, zipf=False):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(T, D, generator=g, device=DEV).to(dtype)
+    logits = torch.randn(T, E, generator=g, device=DEV)
+    if zipf:
+        logits -= 1.1 * torch.log(torch.arange(1, E + 1, device=DEV).float())
+    top, idx = logits.topk(K, 1)
+    ws, ss = zip(*(bw.quantize_expert_weights_int8(torch.randn(E, a, b, generator=g, device=DEV) * 0.02)
+                   for a, b in ((D, H), (D, H), (H, D))))
+    return x, top.softmax(1), idx.to(torch.int32), ws, ss
+
+
+BLOCKS = [(1, 64, 48, 4, 2, BF16, False), (64, 2048, 1408, 64, 6, BF16, False), (37, 256, 400, 16, 4, F16, True),
+          (1003, 512, 768, 128, 8, F16, True), (3000, 256, 512, 8, 2, BF16, False), (300, 128, 16384 + 32, 2, 1, BF16, False)]
+
+
+@pytest.mark.parametrize("T,D,H,E,K,dtype,zipf", BLOCKS)
+def test_block_is_its_operators_in_a_row(T, D, H, E, K, dtype, zipf):
+    x, weights, idx, (wg, wu, wd), (sg, su, sd) = make_block(T, D, H, E, K, dtype, T, zipf)
+    if T > 5:
+        idx[3, 0], idx[4, K - 1] = E, -1            # no expert: contributes nothing
+    out = bw.int8_moe_forward_routed(x, weights, idx, wg, wu, wd, sg, su, sd)
+    rows, plan = bw.permute_tokens(x, idx, E)
+    codes, s = bw.quantize_tokens_int8(rows)
+    assert all(torch.equal(a, b) for a, b in zip((codes, s), bw.quantize_tokens_int8(x, plan)))
+    h = bw.int8_grouped_swiglu(codes, s, plan.offsets, wg, wu, sg, su, out_dtype=dtype)
+    hq, sh = bw.quantize_tokens_int8(h)
+    y = bw.int8_grouped_gemm(hq, sh, plan.offsets, wd, sd, out_dtype=dtype)
+    assert torch.equal(out, bw.unpermute_tokens(y, plan, weights))
+    # and against the definition in 64 bits, h and y rounded to the type.  Where the fp32 h lies next to a border of the
+    # type (2^-20 of the 2^-8 between two bf16 numbers) it may round the other way, and move codes by one: far below the
+    # rounding of the result, half a step at most.
+    ref = torch.zeros(T, D, dtype=torch.float64, device=DEV)
+    for e in range(E):
+        t, k = torch.nonzero(idx == e, as_tuple=True)
+        if len(t) == 0:
+            continue
+        c, sc = (v.to(DEV) for v in exact_codes(x[t]))
+        gate, up = (c.double() @ w[e].double() * sc[:, None].double() * ws[e].double() for w, ws in ((wg, sg), (wu, su)))
+        c, sc = (v.to(DEV) for v in exact_codes((gate * torch.sigmoid(gate) * up).to(dtype)))
+        y64 = (c.double() @ wd[e].double() * sc[:, None].double() * sd[e].double()).to(dtype).double()
+        ref.index_add_(0, t, y64 * weights[t, k, None].double())
+    assert (out.double() - ref).norm() <= ref.norm() * (half_step(dtype) + 1e-3)
+
+
+def test_block_with_its_router():
+    T, D, H, E, K = 130, 256, 512, 16, 2
+    x, _, _, ws, ss = make_block(T, D, H, E, K, BF16, 3)
+    gate = (torch.randn(D, E, device=DEV) * 0.02).to(BF16)
+    out = bw.int8_moe_forward(x, gate, *ws, *ss, top_k=K)
+    assert torch.equal(out, bw.int8_moe_forward_routed(x, *bw.top_k_router(x, gate, K), *ws, *ss))
+
+
+def test_block_beside_the_reference_in_bf16():
+    """Four quantisations (x, gate/up, h, down), each off by scale / sqrt(12) with scale = amax / 127: about 0.9 % where the
+    largest is 4 standard deviations, 2 % for the heavier tails of h.  Together below 4 %."""
+    import oracle
+    from helpers import make_inputs
+    inp = make_inputs(96, 512, 8, 2, 256, seed=2)
+    ref = oracle.moe_forward_bf16(inp["x"], inp["w_gate"], inp["bf_gate"], inp["bf_up"], inp["bf_down"], top_k=2)
+    ws, ss = zip(*(bw.quantize_expert_weights_int8(inp[k].to(DEV)) for k in ("bf_gate", "bf_up", "bf_down")))
+    out = bw.int8_moe_forward(inp["x"].to(DEV), inp["w_gate"].to(DEV), *ws, *ss, top_k=2).cpu()
+    assert oracle.rel_l1(out, ref) < 0.04
+
+
+def test_empty_batches():
+    x, w, idx, ws, ss = make_block(4, 64, 48, 4, 2, BF16, 0)
+    assert bw.int8_moe_forward_routed(x[:0], w[:0], idx[:0], *ws, *ss).shape == (0, 64)
+    assert bw.int8_matmul(x[:0], ws[0][0], ss[0][0]).shape == (0, 48)
+    codes, s = bw.quantize_tokens_int8(x[:0])
+    assert codes.shape == (0, 64) and s.shape == (0,)
+    none = torch.zeros(5, dtype=torch.int32, device=DEV)
+    assert bw.int8_grouped_gemm(codes, s, none, ws[0], ss[0]).shape == (0, 48)
+
+
+@pytest.mark.parametrize("T", [1, 9, 700])
+def test_streams_and_captured_graphs(T):
+    D, H, E, K = 256, 512, 16, 4
+    x, weights, idx, ws, ss = make_block(T, D, H, E, K, BF16, 5)
+
+    def step():
+        return bw.int8_moe_forward_routed(x, weights, idx, *ws, *ss), bw.int8_matmul(x, ws[0][0], ss[0][0])
+
+    want = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step()
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(4):
+        x.normal_()
+        weights.copy_(torch.rand_like(weights))
+        idx.copy_(torch.rand(T, E, device=DEV).topk(K, 1).indices)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+
+
+def test_segments_from_elsewhere_stay_inside_the_rows():
+    """Offsets past the rows, negative or falling: clamped, nothing is read or written out of range."""
+    M, K, N, E = 40, 64, 64, 3
+    a, w = make_codes((M, K), 1).to(DEV), make_codes((E, K, N), 2).to(DEV)
+    rs, cs = torch.ones(M, device=DEV), torch.ones(E, N, device=DEV)
+    for offsets in ([0, 10, 30, 4000], [-7, 10, 30, 40], [0, 2 ** 31 - 1, 30, 40], [40, 10, 5, 0]):
+        out = bw.int8_grouped_gemm(a, rs, torch.tensor(offsets, dtype=torch.int32, device=DEV), w, cs, out_dtype=F32)
+        torch.cuda.synchronize()
+        if offsets[1:3] == [10, 30]:
+            for e, (lo, hi) in enumerate(((0, 10), (10, 30), (30, 40))):
+                assert torch.equal(out[lo:hi].double(), a[lo:hi].double() @ w[e].double())
