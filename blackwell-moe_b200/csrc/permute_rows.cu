@@ -47,6 +47,8 @@ template <class P> __device__ __forceinline__ P zero_piece() {
   return z;
 }
 
+template <int ROWS> constexpr int kPiecesPerThread = ROWS >= 4 ? 8 / ROWS : 2;
+
 // Row of slot s; -1 where there is none.  A plan is data from outside the kernel: an entry past the rows is no row.
 __device__ __forceinline__ int row_of(const int32_t* __restrict__ pos, long long s, int M) {
   const int p = pos[s];
@@ -82,24 +84,28 @@ permute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ x, const int
   }
 }
 
-// Eight rows at a time: their places first, then their pieces, all requested before the first is used.
-template <class T, int BYTES, bool WEIGHTED>
+// R rows at a time and U pieces of each per thread: their places first, then their pieces, all requested before the first
+// is used.  Four to eight pieces in flight per thread, whatever K is (with R = 8 for two rows per token the registers that six absent
+// rows held kept half of the threads off the chip: 137 us for 16384 tokens x 2 rows of 4096, 61 us at the memory's rate).
+template <class T, int BYTES, bool WEIGHTED, int R>
 __global__ void __launch_bounds__(kThreads)
 unpermute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ rows, const int32_t* __restrict__ pos,
                       const float* __restrict__ weights, int n_tok, int K, int pieces, int lanes,
                       typename Piece<BYTES>::type* __restrict__ out) {
-  constexpr int W = BYTES / (int)sizeof(T), R = 8;
+  constexpr int W = BYTES / (int)sizeof(T), U = kPiecesPerThread<R>;
   chain_wait();
-  const int t = blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes, c = blockIdx.y * lanes + threadIdx.x % lanes;
-  if (t >= n_tok || c >= pieces) return;
+  const int t = blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes, c0 = blockIdx.y * lanes * U + threadIdx.x % lanes;
+  if (t >= n_tok || c0 >= pieces) return;
   const int M = n_tok * K;
-  float acc[W];
+  float acc[U][W];
 #pragma unroll
-  for (int i = 0; i < W; ++i) acc[i] = 0.f;
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < W; ++i) acc[u][i] = 0.f;
   for (int k0 = 0; k0 < K; k0 += R) {
     int p[R];
     float w[R];
-    Values<T, BYTES> q[R];
+    Values<T, BYTES> q[R][U];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       p[j] = k0 + j < K ? row_of(pos, (size_t)t * K + k0 + j, M) : -1;
@@ -107,22 +113,31 @@ unpermute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ rows, cons
     }
 #pragma unroll
     for (int j = 0; j < R; ++j)
-      if (p[j] >= 0) q[j].raw = rows[(size_t)p[j] * pieces + c];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (p[j] >= 0 && c0 + u * lanes < pieces) q[j][u].raw = rows[(size_t)p[j] * pieces + c0 + u * lanes];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       if (p[j] < 0) continue;
 #pragma unroll
-      for (int i = 0; i < W; ++i) acc[i] = WEIGHTED ? fmaf(w[j], to_f32(q[j].v[i]), acc[i]) : acc[i] + to_f32(q[j].v[i]);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          acc[u][i] = WEIGHTED ? fmaf(w[j], to_f32(q[j][u].v[i]), acc[u][i]) : acc[u][i] + to_f32(q[j][u].v[i]);
     }
   }
-  Values<T, BYTES> o;
 #pragma unroll
-  for (int i = 0; i < W; ++i) o.v[i] = from_f32<T>(acc[i]);
-  out[(size_t)t * pieces + c] = o.raw;
+  for (int u = 0; u < U; ++u) {
+    if (c0 + u * lanes >= pieces) continue;
+    Values<T, BYTES> o;
+#pragma unroll
+    for (int i = 0; i < W; ++i) o.v[i] = from_f32<T>(acc[u][i]);
+    out[(size_t)t * pieces + c0 + u * lanes] = o.raw;
+  }
 }
 
 // wpt warps (1, 2, 4 or 8) share a token; lane l of them takes every (32 * wpt)-th piece of the row.
-template <class T, int BYTES, bool DROWS, bool DW>
+template <class T, int BYTES, bool DROWS, bool DW, int R>
 __global__ void __launch_bounds__(kThreads)
 unpermute_rows_backward_kernel(const typename Piece<BYTES>::type* __restrict__ dout,
                                const typename Piece<BYTES>::type* __restrict__ rows, const int32_t* __restrict__ pos,
@@ -130,7 +145,7 @@ unpermute_rows_backward_kernel(const typename Piece<BYTES>::type* __restrict__ d
                                int K, int pieces, int wpt, typename Piece<BYTES>::type* __restrict__ drows,
                                float* __restrict__ dweights) {
   using P = typename Piece<BYTES>::type;
-  constexpr int W = BYTES / (int)sizeof(T), R = 8;
+  constexpr int W = BYTES / (int)sizeof(T);
   chain_wait();
   __shared__ float s_part[kThreads / 32][R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -238,13 +253,19 @@ template <class T, int BYTES>
 int run_unpermute(const void* rows, const int32_t* pos, const float* weights, int n_tok, int K, size_t row_bytes, void* out,
                   cudaStream_t st) {
   using P = typename Piece<BYTES>::type;
-  const int pieces = (int)(row_bytes / BYTES), lanes = lanes_for(pieces);
-  const dim3 grid((unsigned)ceil_div(n_tok, kThreads / lanes), (unsigned)ceil_div(pieces, lanes));
-  BWMOE_REQUIRE(grid.y <= 65535, BWMOE_ERR_UNSUPPORTED, "unpermute_rows: rows of %zu bytes", row_bytes);
-  auto kernel = weights ? unpermute_rows_kernel<T, BYTES, true> : unpermute_rows_kernel<T, BYTES, false>;
-  BWMOE_CUDA_OK(launch_chained(kernel, grid, dim3(kThreads), 0, st, static_cast<const P*>(rows), pos, weights, n_tok, K,
-                               pieces, lanes, static_cast<P*>(out)));
-  return BWMOE_OK;
+  const int pieces = (int)(row_bytes / BYTES);
+  auto run = [&](auto rows_at_once) {
+    constexpr int R = decltype(rows_at_once)::value, U = kPiecesPerThread<R>;
+    const int lanes = lanes_for(ceil_div(pieces, U));
+    const dim3 grid((unsigned)ceil_div(n_tok, kThreads / lanes), (unsigned)ceil_div(pieces, U * lanes));
+    BWMOE_REQUIRE(grid.y <= 65535, BWMOE_ERR_UNSUPPORTED, "unpermute_rows: rows of %zu bytes", row_bytes);
+    auto kernel = weights ? unpermute_rows_kernel<T, BYTES, true, R> : unpermute_rows_kernel<T, BYTES, false, R>;
+    BWMOE_CUDA_OK(launch_chained(kernel, grid, dim3(kThreads), 0, st, static_cast<const P*>(rows), pos, weights, n_tok, K,
+                                 pieces, lanes, static_cast<P*>(out)));
+    return (int)BWMOE_OK;
+  };
+  return K <= 2 ? run(std::integral_constant<int, 2>{}) : K <= 4 ? run(std::integral_constant<int, 4>{})
+                                                                 : run(std::integral_constant<int, 8>{});
 }
 
 template <class T, int BYTES>
@@ -257,13 +278,18 @@ int run_unpermute_backward(const void* dout, const void* rows, const int32_t* po
   int wpt = 1;
   while (wpt < 8 && 32 * wpt < pieces && (long long)n_tok * wpt < 16ll * sm_count()) wpt *= 2;
   const unsigned blocks = (unsigned)ceil_div(n_tok, kThreads / 32 / wpt);
-  auto kernel = drows && dweights ? unpermute_rows_backward_kernel<T, BYTES, true, true>
-                : drows           ? unpermute_rows_backward_kernel<T, BYTES, true, false>
-                                  : unpermute_rows_backward_kernel<T, BYTES, false, true>;
-  BWMOE_CUDA_OK(launch_chained(kernel, dim3(blocks), dim3(kThreads), 0, st, static_cast<const P*>(dout),
-                               static_cast<const P*>(rows), pos, offsets, E, weights, n_tok, K, pieces, wpt,
-                               static_cast<P*>(drows), dweights));
-  return BWMOE_OK;
+  auto run = [&](auto rows_at_once) {
+    constexpr int R = decltype(rows_at_once)::value;
+    auto kernel = drows && dweights ? unpermute_rows_backward_kernel<T, BYTES, true, true, R>
+                  : drows           ? unpermute_rows_backward_kernel<T, BYTES, true, false, R>
+                                    : unpermute_rows_backward_kernel<T, BYTES, false, true, R>;
+    BWMOE_CUDA_OK(launch_chained(kernel, dim3(blocks), dim3(kThreads), 0, st, static_cast<const P*>(dout),
+                                 static_cast<const P*>(rows), pos, offsets, E, weights, n_tok, K, pieces, wpt,
+                                 static_cast<P*>(drows), dweights));
+    return (int)BWMOE_OK;
+  };
+  return K <= 2 ? run(std::integral_constant<int, 2>{}) : K <= 4 ? run(std::integral_constant<int, 4>{})
+                                                                 : run(std::integral_constant<int, 8>{});
 }
 
 // fn(type tag, piece tag) for the element type and the widest piece

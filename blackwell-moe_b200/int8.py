@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .moe import _contig, _require_cuda, _stream, _workspace
+from .moe import _contig, _on_device, _require_cuda, _stream, _workspace
 from .permute import _DTYPES, _check_plan, _dtype_code
 
 _I8 = torch.int8
@@ -47,7 +47,7 @@ def quantize_tokens_int8(x: torch.Tensor, plan=None):
     codes = torch.empty((T * K, D), dtype=_I8, device=dev)
     scales = torch.empty(T * K, dtype=torch.float32, device=dev)
     if T:
-        with torch.cuda.device(dev):
+        with _on_device(dev):
             _lib.check(_lib.lib().bwmoe_int_quant(x.data_ptr(), pos.data_ptr() if plan is not None else None,
                                                   offsets.data_ptr() if plan is not None else None, T, D, E, K, code,
                                                   codes.data_ptr(), scales.data_ptr(), _stream(dev)))
@@ -75,7 +75,7 @@ def _grouped(fn_name, codes, scales, offsets, weights, w_scales, out_dtype):
     out = torch.empty((M, N), dtype=out_dtype, device=dev)
     if M:
         lib = _lib.lib()
-        with torch.cuda.device(dev):
+        with _on_device(dev):
             ws = _workspace(dev, lib.bwmoe_int_scratch_bytes(M, D, N, E))
             _lib.check(getattr(lib, fn_name)(codes.data_ptr(), scales.data_ptr(), offsets.data_ptr(),
                                              *[w.data_ptr() for w in weights], *[s.data_ptr() for s in w_scales], M, D, N, E,
@@ -105,7 +105,7 @@ def int8_matmul(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor) -> tor
     if T == 0:
         return out
     lib = _lib.lib()
-    with torch.cuda.device(dev):
+    with _on_device(dev):
         need = lib.bwmoe_workspace_bytes_int_matmul(T, K, N)
         if need == 0:
             raise ValueError(f"unsupported shape T={T} K={K} N={N} (K and N must be multiples of 16)")
@@ -152,7 +152,7 @@ def int8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, e
     weights, indices = (_contig(t, "routing") for t in (router_weights.to(torch.float32), expert_indices.to(torch.int32)))
     _require_cuda(x, weights, indices)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
+    with _on_device(dev):
         out = torch.empty_like(x)
         if T == 0:
             return out
@@ -172,7 +172,7 @@ def int8_moe_forward(x, w_gate, experts_w_gate, experts_w_up, experts_w_down, sc
     assert w_gate.shape == (D, E) and w_gate.dtype == torch.bfloat16, (w_gate.shape, w_gate.dtype)
     _require_cuda(x, _contig(w_gate, "w_gate"))
     lib = _lib.lib()
-    with torch.cuda.device(dev):
+    with _on_device(dev):
         out = torch.empty_like(x)
         if T == 0:
             return out

@@ -9,6 +9,7 @@ device memory and streams only.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -37,8 +38,22 @@ def _contig(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
+# the current stream's handle without the Stream object around it (2 us of every call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    if _raw_stream is None or dev.index is None:
+        return torch.cuda.current_stream(dev).cuda_stream
+    return _raw_stream(dev.index)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on_device(dev):
+    """``torch.cuda.device(dev)`` for the launches of a call; nothing to do where it is the current device already."""
+    return _SAME_DEVICE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _workspace(dev, nbytes: int) -> torch.Tensor:
@@ -72,7 +87,7 @@ def top_k_router(hidden: torch.Tensor, gate_w: torch.Tensor, k: int, *, as_batch
     E = gate_w.shape[1]
     hidden, gate_w = _contig(hidden, "hidden"), _contig(gate_w, "gate_w")
     lib = _lib.lib()
-    with torch.cuda.device(dev):
+    with _on_device(dev):
         w_out = torch.empty((T, k), device=dev, dtype=torch.float32)
         i_out = torch.empty((T, k), device=dev, dtype=torch.int32)
         t_as = int(as_batch) if as_batch else 0
@@ -135,7 +150,7 @@ def fp8_moe_forward(x, w_gate, experts_w_gate, experts_w_up, experts_w_down,
     dev = _require_cuda(*weights)
     lib = _lib.lib()
     x = _contig(x, "x")
-    with torch.cuda.device(dev):
+    with _on_device(dev):
         ptrs = [t.data_ptr() for t in weights]
         if routed_scale != 1.0 or residual is not None:
             if scales_gate.dim() == 3 or not x.is_cuda:
@@ -208,7 +223,7 @@ def fp8_moe_forward_shared(x, w_gate, experts_w_gate, experts_w_up, experts_w_do
                                               scales_gate, scales_up, scales_down)]
     dev = _require_cuda(*tensors)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
+    with _on_device(dev):
         need = lib.bwmoe_workspace_bytes_shared(T, D, H, E, top_k, n_shared)
         if need == 0:
             raise ValueError(f"unsupported shape T={T} D={D} H={H} E={E}+{n_shared} top_k={top_k}+{n_shared}")
@@ -268,7 +283,7 @@ def fp8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, ex
         _require_cuda(x, remap)
         n_total = remap.numel()
     lib = _lib.lib()
-    with torch.cuda.device(dev):
+    with _on_device(dev):
         need = (lib.bwmoe_workspace_bytes_block if block else lib.bwmoe_workspace_bytes)(T, D, H, E, K)
         if need == 0:
             raise ValueError(f"unsupported shape T={T} D={D} H={H} E={E} top_k={K}")

@@ -14,7 +14,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .moe import _contig, _require_cuda, _stream
+from .moe import _contig, _on_device, _require_cuda, _stream
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -38,10 +38,13 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _empty_plan(T, K, num_experts, dev):
-    M = T * K
-    o, p, s, e = torch.empty(num_experts + 1 + 3 * M, dtype=torch.int32, device=dev).split((num_experts + 1, M, M, M))
-    return PermutePlan(o, p.view(T, K), s, e)
+def _empty_plan(T, K, num_experts, scratch_bytes, dev):
+    """The plan's tensors, and the addresses of its status word and scratch behind them: one allocation."""
+    M, extra = T * K, 4 + (scratch_bytes + 3) // 4
+    o, p, s, e, rest = torch.empty(num_experts + 1 + 3 * M + extra, dtype=torch.int32, device=dev).split(
+        (num_experts + 1, M, M, M, extra))
+    status = rest.data_ptr()
+    return PermutePlan(o, p.view(T, K), s, e), status, status + 16
 
 
 def _check_indices(indices, num_experts):
@@ -60,108 +63,128 @@ def _check_plan(plan, name="plan"):
     return offsets, pos
 
 
-def _plan_scratch(lib, T, E, K, dev):
-    # the plan's scratch, and a status word behind it
-    n = lib.bwmoe_plan_scratch_bytes(T, E, K)
-    ws = torch.empty(n + 16, dtype=torch.uint8, device=dev)
-    return ws, n
-
-
 def permute_plan(indices: torch.Tensor, num_experts: int) -> PermutePlan:
     """The stable sort of all slots of ``indices[T,K]`` int32 by expert id."""
     indices = _check_indices(indices, num_experts)
     dev = _require_cuda(indices)
     T, K = indices.shape
-    with torch.cuda.device(dev):
-        plan = _empty_plan(T, K, num_experts, dev)
+    lib = _lib.lib()
+    with _on_device(dev):
+        plan, status, scratch = _empty_plan(T, K, num_experts, lib.bwmoe_plan_scratch_bytes(T, num_experts, K), dev)
         if T == 0:
             plan.offsets.zero_()
             return plan
-        lib = _lib.lib()
-        ws, n = _plan_scratch(lib, T, num_experts, K, dev)
-        _lib.check(lib.bwmoe_permute_plan(indices.data_ptr(), None, T, num_experts, K, *[t.data_ptr() for t in plan], None,
-                                          ws.data_ptr() + n, ws.data_ptr(), _stream(dev)))
+        _lib.check(lib.bwmoe_permute_plan(indices.data_ptr(), None, T, num_experts, K, plan.offsets.data_ptr(),
+                                          plan.pos.data_ptr(), plan.row_slot.data_ptr(), plan.row_expert.data_ptr(), None,
+                                          status, scratch, _stream(dev)))
     return plan
 
 
-def _permute(x, plan):
+def _permute_new(x, indices, num_experts):
+    """The plan and the rows in one call."""
+    T, K = indices.shape
+    D, dev = x.shape[1], x.device
+    lib = _lib.lib()
+    with _on_device(dev):
+        plan, status, scratch = _empty_plan(T, K, num_experts, lib.bwmoe_plan_scratch_bytes(T, num_experts, K), dev)
+        rows = torch.empty((T * K, D), dtype=x.dtype, device=dev)
+        pos = plan.pos.data_ptr()
+        _lib.check(lib.bwmoe_permute_tokens(x.data_ptr(), indices.data_ptr(), T, D, num_experts, K, _DTYPES[x.dtype],
+                                            plan.offsets.data_ptr(), pos, pos + 4 * T * K, pos + 8 * T * K, rows.data_ptr(),
+                                            status, scratch, _stream(dev)))
+    return rows, plan
+
+
+def _permute(x, offsets, pos):
     """rows[pos[t,k]] = x[t]"""
-    T, K = plan.pos.shape
-    rows = torch.empty((T * K, x.shape[1]), dtype=x.dtype, device=x.device)
-    if rows.numel():
-        with torch.cuda.device(x.device):
-            _lib.check(_lib.lib().bwmoe_permute_rows(x.data_ptr(), plan.pos.data_ptr(), plan.offsets.data_ptr(), T, x.shape[1],
-                                                     plan.offsets.numel() - 1, K, _DTYPES[x.dtype], rows.data_ptr(),
-                                                     _stream(x.device)))
+    T, K = pos.shape
+    D, dev = x.shape[1], x.device
+    with _on_device(dev):
+        rows = torch.empty((T * K, D), dtype=x.dtype, device=dev)
+        if T and D:
+            _lib.check(_lib.lib().bwmoe_permute_rows(x.data_ptr(), pos.data_ptr(), offsets.data_ptr(), T, D, offsets.numel() - 1,
+                                                     K, _DTYPES[x.dtype], rows.data_ptr(), _stream(dev)))
     return rows
 
 
 def _unpermute(rows, pos, weights):
     """sum over k of w[t,k] * rows[pos[t,k]]"""
     T, K = pos.shape
-    out = torch.empty((T, rows.shape[1]), dtype=rows.dtype, device=rows.device)
-    if out.numel():
-        with torch.cuda.device(rows.device):
+    D, dev = rows.shape[1], rows.device
+    with _on_device(dev):
+        out = torch.empty((T, D), dtype=rows.dtype, device=dev)
+        if T and D:
             _lib.check(_lib.lib().bwmoe_unpermute_rows(rows.data_ptr(), pos.data_ptr(),
-                                                       None if weights is None else weights.data_ptr(), T, rows.shape[1], K,
-                                                       _DTYPES[rows.dtype], out.data_ptr(), _stream(rows.device)))
+                                                       None if weights is None else weights.data_ptr(), T, D, K,
+                                                       _DTYPES[rows.dtype], out.data_ptr(), _stream(dev)))
     return out
 
 
+def _unpermute_backward(dout, rows, offsets, pos, weights, rows_grad, weights_grad):
+    T, K = pos.shape
+    D, dev = dout.shape[1], dout.device
+    with _on_device(dev):
+        drows = torch.empty((T * K, D), dtype=dout.dtype, device=dev) if rows_grad else None
+        dweights = torch.empty((T, K), dtype=torch.float32, device=dev) if weights_grad else None
+        if T and D:
+            if rows_grad or weights_grad:
+                _lib.check(_lib.lib().bwmoe_unpermute_rows_backward(
+                    dout.data_ptr(), rows.data_ptr() if weights_grad else None, pos.data_ptr(), offsets.data_ptr(),
+                    weights.data_ptr(), T, D, offsets.numel() - 1, K, _DTYPES[dout.dtype], drows.data_ptr() if rows_grad else None,
+                    dweights.data_ptr() if weights_grad else None, _stream(dev)))
+        elif weights_grad:
+            dweights.zero_()
+    return drows, dweights
+
+
+def _once(backward):
+    """``once_differentiable`` where a second derivative could be asked for (``create_graph``): its bookkeeping costs as
+    much as a small batch's backward pass."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+    return staticmethod(lambda ctx, grad: guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad))
+
+
+def _permute_backward(ctx, drows):
+    return _unpermute(drows.contiguous(), ctx.saved_tensors[0], None), None, None
+
+
 class _PermuteRows(torch.autograd.Function):
+    backward = _once(_permute_backward)
+
     @staticmethod
     def forward(ctx, x, offsets, pos):
         ctx.save_for_backward(pos)
-        return _permute(x, PermutePlan(offsets, pos, None, None))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, drows):
-        return _unpermute(drows.contiguous(), ctx.saved_tensors[0], None), None, None
+        return _permute(x, offsets, pos)
 
 
 class _PermuteTokens(torch.autograd.Function):
-    """The plan and the rows in one call."""
+    backward = _once(_permute_backward)
 
     @staticmethod
-    def forward(ctx, x, indices, num_experts):
-        T, K = indices.shape
-        D, dev = x.shape[1], x.device
-        plan = _empty_plan(T, K, num_experts, dev)
-        rows = torch.empty((T * K, D), dtype=x.dtype, device=dev)
-        lib = _lib.lib()
-        with torch.cuda.device(dev):
-            ws, n = _plan_scratch(lib, T, num_experts, K, dev)
-            _lib.check(lib.bwmoe_permute_tokens(x.data_ptr(), indices.data_ptr(), T, D, num_experts, K, _DTYPES[x.dtype],
-                                                *[t.data_ptr() for t in plan], rows.data_ptr(), ws.data_ptr() + n,
-                                                ws.data_ptr(), _stream(dev)))
+    def forward(ctx, x, args, found):        # args: (indices, num_experts); the plan leaves through the list `found`
+        rows, plan = _permute_new(x, *args)
         ctx.save_for_backward(plan.pos)
-        ctx.mark_non_differentiable(*plan)
-        return (rows, *plan)
+        found.append(plan)
+        return rows
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, drows, *_):
-        return _unpermute(drows.contiguous(), ctx.saved_tensors[0], None), None, None
+
+def _unpermute_rows_backward(ctx, dout):
+    rows, offsets, pos, weights = ctx.saved_tensors
+    dout = dout.contiguous()
+    if weights is None:
+        return _permute(dout, offsets, pos), None, None, None
+    drows, dweights = _unpermute_backward(dout, rows, offsets, pos, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[3])
+    return drows, None, None, dweights
 
 
 class _UnpermuteRows(torch.autograd.Function):
+    backward = _once(_unpermute_rows_backward)
+
     @staticmethod
     def forward(ctx, rows, offsets, pos, weights):
         # the rows are kept for the weights' gradient only
         ctx.save_for_backward(rows if ctx.needs_input_grad[3] else None, offsets, pos, weights)
         return _unpermute(rows, pos, weights)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        rows, offsets, pos, weights = ctx.saved_tensors
-        dout = dout.contiguous()
-        if weights is None:
-            return _permute(dout, PermutePlan(offsets, pos, None, None)), None, None, None
-        drows, dweights = unpermute_tokens_backward(dout, rows, PermutePlan(offsets, pos, None, None), weights,
-                                                    rows_grad=ctx.needs_input_grad[0], weights_grad=ctx.needs_input_grad[3])
-        return drows, None, None, dweights
 
 
 def permute_tokens(x: torch.Tensor, indices: torch.Tensor = None, num_experts: int = None, *, plan: PermutePlan = None):
@@ -169,23 +192,25 @@ def permute_tokens(x: torch.Tensor, indices: torch.Tensor = None, num_experts: i
     (stable).  ``indices[T,K]`` int32 are the tokens' experts; or pass the ``plan`` of an earlier call.  Rows that no slot
     owns are zero.  The gradient of a token is the sum of its rows' gradients."""
     assert x.dim() == 2, x.shape
-    code = _dtype_code(x, "x")
-    x = _contig(x, "x")
+    _dtype_code(x, "x")
+    _contig(x, "x")
     if (indices is None) == (plan is None) or (indices is None) != (num_experts is None):
         raise ValueError("permute_tokens takes indices and num_experts, or a plan")
-    if plan is not None:
-        offsets, pos = _check_plan(plan)
-        assert pos.shape[0] == x.shape[0], (pos.shape, x.shape)
-        _require_cuda(x, offsets, pos)
-        return _PermuteRows.apply(x, offsets, pos), plan
-    indices = _check_indices(indices, num_experts)
-    assert indices.shape[0] == x.shape[0], (indices.shape, x.shape)
-    _require_cuda(x, indices)
-    if x.numel() == 0:
+    wants_grad = x.requires_grad and torch.is_grad_enabled()
+    if plan is None:
+        _check_indices(indices, num_experts)
+        assert indices.shape[0] == x.shape[0], (indices.shape, x.shape)
+        _require_cuda(x, indices)
+        if x.numel():
+            if not wants_grad:
+                return _permute_new(x, indices, num_experts)
+            found = []
+            return _PermuteTokens.apply(x, (indices, num_experts), found), found[0]
         plan = permute_plan(indices, num_experts)
-        return _PermuteRows.apply(x, plan.offsets, plan.pos), plan
-    rows, *parts = _PermuteTokens.apply(x, indices, num_experts)
-    return rows, PermutePlan(*parts)
+    offsets, pos = _check_plan(plan)
+    assert pos.shape[0] == x.shape[0], (pos.shape, x.shape)
+    _require_cuda(x, offsets, pos)
+    return (_PermuteRows.apply(x, offsets, pos) if wants_grad else _permute(x, offsets, pos)), plan
 
 
 def _check_unpermute(rows, plan, weights):
@@ -205,7 +230,9 @@ def unpermute_tokens(rows: torch.Tensor, plan: PermutePlan, weights: torch.Tenso
     """``rows[T*K,D]`` in expert order -> ``out[T,D]``, ``out[t] = sum_k weights[t,k] * rows[plan.pos[t,k]]`` with
     ``weights[T,K]`` fp32 (absent: 1).  Slots without a row add nothing.  Differentiable in ``rows`` and ``weights``."""
     offsets, pos = _check_unpermute(rows, plan, weights)
-    return _UnpermuteRows.apply(rows, offsets, pos, weights)
+    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+        return _UnpermuteRows.apply(rows, offsets, pos, weights)
+    return _unpermute(rows, pos, weights)
 
 
 def unpermute_tokens_backward(dout: torch.Tensor, rows: torch.Tensor, plan: PermutePlan, weights: torch.Tensor, *,
@@ -213,9 +240,9 @@ def unpermute_tokens_backward(dout: torch.Tensor, rows: torch.Tensor, plan: Perm
     """The gradients of :func:`unpermute_tokens` without autograd, for programs that run (or capture) their backward pass
     themselves: ``(drows, dweights)``, ``None`` where not asked for.  ``rows`` may be ``None`` without ``weights_grad``."""
     assert dout.dim() == 2, dout.shape
-    code = _dtype_code(dout, "dout")
+    _dtype_code(dout, "dout")
     offsets, pos = _check_plan(plan)
-    (T, K), D, dev = pos.shape, dout.shape[1], dout.device
+    (T, K), D = pos.shape, dout.shape[1]
     assert dout.shape[0] == T, (dout.shape, pos.shape)
     assert weights.shape == pos.shape and weights.dtype == torch.float32, (weights.shape, weights.dtype)
     tensors = [_contig(dout, "dout"), offsets, pos, _contig(weights, "weights")]
@@ -223,14 +250,4 @@ def unpermute_tokens_backward(dout: torch.Tensor, rows: torch.Tensor, plan: Perm
         assert rows is not None and rows.shape == (T * K, D) and rows.dtype == dout.dtype, (None if rows is None else rows.shape)
         tensors.append(_contig(rows, "rows"))
     _require_cuda(*tensors)
-    drows = torch.empty((T * K, D), dtype=dout.dtype, device=dev) if rows_grad else None
-    dweights = torch.empty((T, K), dtype=torch.float32, device=dev) if weights_grad else None
-    if T == 0 or D == 0:
-        return drows, (dweights.zero_() if weights_grad else None)
-    if rows_grad or weights_grad:
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().bwmoe_unpermute_rows_backward(
-                dout.data_ptr(), rows.data_ptr() if weights_grad else None, pos.data_ptr(), offsets.data_ptr(),
-                weights.data_ptr(), T, D, offsets.numel() - 1, K, code, drows.data_ptr() if rows_grad else None,
-                dweights.data_ptr() if weights_grad else None, _stream(dev)))
-    return drows, dweights
+    return _unpermute_backward(dout, rows, offsets, pos, weights, rows_grad, weights_grad)
