@@ -334,8 +334,8 @@ bool make_int8_layout(int T, int D, int H, int E, int K, Int8Layout* L) {
   };
   L->status = take(16);
   L->router_head = take(kRouterHeadBytes);
-  L->zero_end = o;
-  L->gemm_scratch = take(int8_scratch_bytes((int)M, std::max(D, H), std::max(D, H), E));
+  L->gemm_scratch = take(std::max(int8_scratch_bytes((int)M, D, H, E), int8_scratch_bytes((int)M, H, D, E)));   // for both products
+  L->zero_end = L->gemm_scratch + int8_clear_bytes();
   L->offsets = take(sizeof(int32_t) * (E + 1));
   L->topk_idx = take(sizeof(int32_t) * M);
   L->topk_w = take(sizeof(float) * M);
@@ -386,12 +386,13 @@ int run_int8_pipeline(const void* x, const float* weights, const int32_t* indice
                         nullptr, status, at<void>(ws, L.plan_scratch), st)))
     return rc;
   if ((rc = launch_quant_int8_rows(x, pos, offsets, T, D, E, K, dtype, at<void>(ws, L.xq), sx, st))) return rc;
-  if ((rc = launch_int8_gemm(at<void>(ws, L.xq), sx, offsets, wg, wu, sg, su, M, D, H, E, dtype, at<void>(ws, L.h), status, st)))
+  if ((rc = launch_int8_gemm(at<void>(ws, L.xq), sx, offsets, wg, wu, sg, su, M, D, H, E, dtype, at<void>(ws, L.h),
+                             at<void>(ws, L.gemm_scratch), st, false, status)))
     return rc;
   if ((rc = launch_quant_int8_rows(at<void>(ws, L.h), nullptr, nullptr, M, H, 1, 1, dtype, at<void>(ws, L.hq), sh, st)))
     return rc;
   if ((rc = launch_int8_gemm(at<void>(ws, L.hq), sh, offsets, wd, nullptr, sd, nullptr, M, H, D, E, dtype, at<void>(ws, L.y),
-                             status, st)))
+                             at<void>(ws, L.gemm_scratch), st, false, status)))
     return rc;
   return launch_unpermute_rows(at<void>(ws, L.y), pos, weights, T, D, K, dtype, out, st);
 }
@@ -920,7 +921,7 @@ int bwmoe_int_grouped_gemm(const void* codes, const float* row_scale, const int3
                             int M, int K, int N, int E, int dtype, void* out, void* scratch, size_t scratch_bytes, void* stream) {
   if (int rc = check_int8_scratch("int_grouped_gemm", M, K, N, E, scratch, scratch_bytes)) return rc;
   return launch_int8_gemm(codes, row_scale, offsets, w, nullptr, scale, nullptr, M, K, N, E, dtype, out,
-                          static_cast<int32_t*>(scratch), static_cast<cudaStream_t>(stream), true);
+                          scratch, static_cast<cudaStream_t>(stream), true);
 }
 
 int bwmoe_int_gateup_swiglu(const void* codes, const float* row_scale, const int32_t* offsets, const void* wg, const void* wu,
@@ -928,7 +929,7 @@ int bwmoe_int_gateup_swiglu(const void* codes, const float* row_scale, const int
                              size_t scratch_bytes, void* stream) {
   if (int rc = check_int8_scratch("int_gateup_swiglu", M, K, N, E, scratch, scratch_bytes)) return rc;
   BWMOE_REQUIRE(wu != nullptr, BWMOE_ERR_NULL, "int_gateup_swiglu: null pointer");
-  return launch_int8_gemm(codes, row_scale, offsets, wg, wu, sg, su, M, K, N, E, dtype, h, static_cast<int32_t*>(scratch),
+  return launch_int8_gemm(codes, row_scale, offsets, wg, wu, sg, su, M, K, N, E, dtype, h, scratch,
                           static_cast<cudaStream_t>(stream), true);
 }
 
@@ -949,10 +950,11 @@ int bwmoe_int_matmul(const void* x, const void* w, const float* scale, int T, in
   if (int rc = check_int8_gemm(at<void>(ws, codes), at<float>(ws, scales), nullptr, w, nullptr, scale, nullptr, T, K, N, 1, dtype, out,
                                at<int32_t>(ws, 0)))
     return rc;
-  if (int rc = launch_quant_int8_rows(x, nullptr, nullptr, T, K, 1, 1, dtype, at<void>(ws, codes), at<float>(ws, scales), st, ws, 16))
+  if (int rc = launch_quant_int8_rows(x, nullptr, nullptr, T, K, 1, 1, dtype, at<void>(ws, codes), at<float>(ws, scales), st, ws,
+                                      int8_clear_bytes()))
     return rc;
   return launch_int8_gemm(at<void>(ws, codes), at<float>(ws, scales), nullptr, w, nullptr, scale, nullptr, T, K, N, 1, dtype, out,
-                          at<int32_t>(ws, 0), st);
+                          ws, st);
 }
 
 size_t bwmoe_workspace_bytes_int(int T, int D, int H, int E, int K) {

@@ -297,14 +297,17 @@ int launch_unpermute_rows_backward(const void* dout, const void* rows, const int
 // Experts in 8-bit integers (quant_int8.cu, grouped_gemm_int8_sm100.cu).  zero: words to be cleared on the way.
 int launch_quant_int8_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
                            void* codes, float* scales, cudaStream_t st, void* zero = nullptr, size_t zero_bytes = 0);
+// Scratch of a product: int8_scratch_bytes(); its first int8_clear_bytes() are zero when the kernel starts (`clear`: zeroed by
+// the call) and begin with the status word, unless `status` names another.
 size_t int8_scratch_bytes(int M, int K, int N, int E);
+size_t int8_clear_bytes();
 // w1 == nullptr: one product; otherwise SwiGLU of the two.  offsets == nullptr: one segment (E = 1).
 int check_int8_gemm(const void* a, const float* row_scale, const int32_t* offsets, const void* w0, const void* w1,
                     const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, const void* out,
                     const int32_t* status);
 int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offsets, const void* w0, const void* w1,
-                     const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, void* out, int32_t* status,
-                     cudaStream_t st, bool clear_status = false);
+                     const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, void* out, void* scratch,
+                     cudaStream_t st, bool clear = false, int32_t* status = nullptr);
 
 // Monotone map of a float onto unsigned integers (a < b  <=>  key(a) < key(b); -0 is folded onto +0 first).
 __device__ __forceinline__ unsigned order_key(float v) {

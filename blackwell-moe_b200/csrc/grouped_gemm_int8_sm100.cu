@@ -7,12 +7,23 @@
 // are exact whatever their order (|a|, |w| <= 128 and K < 2^17); scales, SwiGLU and the one rounding to the output type
 // happen in fp32 in the epilogue.
 //
-// Structure per CTA (320 threads, one CTA per SM, persistent): warp 0 TMA producer, warp 1 tcgen05.mma issuer
-// (kind::i8, M=128 N=256 K=32, int32 accumulators in tensor memory, two 256-column buffers), warps 2..9 epilogue, two per
-// tensor-memory lane quarter.  A tile is 128 rows of one expert x 256 accumulator columns (SWIGLU: 128 gate + 128 up
-// columns); activations are read K-major, weights in the caller's [E, K, N] layout (N contiguous).  Tiles are ordered by
-// expert, then column block, then row block, so that an expert's rows stay in L2 while its weights stream through once.
+// Two kernels, persistent, one CTA per SM, warp-specialised (TMA producer, tcgen05.mma kind::i8 issuer, epilogue warps);
+// activations are read K-major, weights in the caller's [E, K, N] layout (N contiguous):
+//   int8_gemm_kernel        128 rows x 256 channels per tile, the rows on the MMA's M side
+//   int8_gemm_small_kernel  32 rows x 256 channels per tile, the channels on the M side (decode batches)
+// (SWIGLU: 128 gate + 128 up channels in the place of the 256.)
+//
+// Pieces.  Where the tiles do not fill the chip, their K loops are cut into slices.  A slice leaves its accumulators in the
+// scratch, and the one of a tile that arrives last (a counter per tile and epilogue warp) adds them up and finishes the tile:
+// nobody waits for anybody, no second kernel runs, and 32-bit integer sums are the same in every order.  Pieces (tile, slice)
+// are ordered by expert, then slice, then channels, then rows, so that neighbouring CTAs read neighbouring bytes of the same
+// rows of the weights at the same time and an expert's rows stay in L2 while its weights stream through once.  (Dealing the K
+// blocks of all tiles out in equal contiguous shares instead, which keeps every CTA equally busy, reads scattered 256-byte
+// pieces: 4.1 TB/s against 5.6 at 8 experts of 4096 x 14336.)
+//
 // Every wait is bounded as in the other GEMM kernels of this library.
+#include <type_traits>
+
 #include "sm100_gemm.cuh"
 
 namespace bwmoe {
@@ -22,6 +33,7 @@ using namespace sm100;
 // D = int32, A = B = signed 8-bit, A K-major, B MN-major, N = 256, M = 128
 constexpr uint32_t IDESC_I8 = (2u << 4) | (1u << 7) | (1u << 10) | (0u << 15) | (1u << 16) | ((uint32_t)(BN >> 3) << 17) |
                               ((uint32_t)(BM >> 4) << 24);
+constexpr uint32_t IDESC_I8_HALF = (IDESC_I8 & ~(0x3fu << 17)) | ((uint32_t)(BN_HALF >> 3) << 17);      // N = 128: one weight box
 constexpr int kMaxGroups = 256;
 constexpr int EPI_WARPS = 8;
 constexpr int I8_THREADS = 64 + 32 * EPI_WARPS;
@@ -51,7 +63,7 @@ __device__ __forceinline__ void segment(const I8Params& p, int e, int& r0, int& 
   r1 = p.offsets != nullptr ? min(max(p.offsets[e + 1], r0), p.M) : p.M;
 }
 
-// s_first[0 .. E] and s_end[0 .. E-1]: the segments; s_cum[0 .. E]: tiles before each.  All threads of the block.
+// first / end: the segments; cum: tiles before each.  All threads of the block; read behind the next __syncthreads().
 template <int THREADS>
 __device__ __forceinline__ void tile_table(const I8Params& p, int tile_rows, int tiles_per_row_block, int* s_first, int* s_end,
                                            int* s_cum) {
@@ -81,21 +93,90 @@ __device__ __forceinline__ void tile_table(const I8Params& p, int tile_rows, int
   }
 }
 
-// tile index -> (expert, first row, end of its segment, column block); every role walks the same rising sequence
-struct I8Cursor {
+// K blocks per slice (one warp).  In ns, a slicing takes the longer of all K blocks at the memory's rate (32 KiB of weights in
+// 5.5) and of the longest CTA's blocks (one takes an SM about 500), and then the adding up: fixed, and per slice.
+__device__ __forceinline__ int blocks_per_slice(int tiles, int k_blocks, int ctas, int max_pieces, int fixed_ns, int slice_ns) {
+  const int lane = threadIdx.x & 31, per = (k_blocks + lane) / (lane + 1), slices = (k_blocks + per - 1) / per;
+  const long long pieces = (long long)tiles * slices;
+  unsigned cost = 0x7ffffffu;
+  if (slices == 1 || pieces <= max_pieces) {
+    const long long memory = (long long)tiles * k_blocks * 11 / 2, longest = (pieces + ctas - 1) / ctas * per * 500;
+    cost = (unsigned)min((memory > longest ? memory : longest) + (slices > 1 ? fixed_ns + slice_ns * slices : 0), 0x7fffffell);
+  }
+  const unsigned best = __reduce_min_sync(0xffffffffu, cost * 32u + (unsigned)lane);      // (a tie: fewer slices)
+  return __shfl_sync(0xffffffffu, per, best & 31u);
+}
+
+// The pieces' places: every role of a CTA walks the same rising sequence of piece numbers.
+struct I8Pieces {
   const int *first, *end, *cum;
-  int E, tile_rows, e;
-  __device__ bool locate(int tile, int& row0, int& row_end, int& n_idx) {
-    while (e < E && tile >= cum[e + 1]) ++e;
-    if (e >= E) return false;
-    const int m_tiles = (end[e] - first[e] + tile_rows - 1) / tile_rows;
-    const int within = tile - cum[e];
+  int E, tile_rows, k_blocks, per, slices, e;
+  long long total;
+  int tile, row0, row_end, n_idx, slice, kb0, kb1;      // of the piece last located, an expert e's
+  __device__ __forceinline__ I8Pieces(const int* first_, const int* end_, const int* cum_, int E_, int tile_rows_, int k_blocks_, int per_)
+      : first(first_), end(end_), cum(cum_), E(E_), tile_rows(tile_rows_), k_blocks(k_blocks_), per(per_),
+        slices((k_blocks_ + per_ - 1) / per_), e(0), total((long long)cum_[E_] * slices) {}
+  __device__ __forceinline__ void locate(long long piece) {      // piece < total
+    while (piece >= (long long)cum[e + 1] * slices) ++e;
+    const int tiles = cum[e + 1] - cum[e], m_tiles = (end[e] - first[e] + tile_rows - 1) / tile_rows;
+    int within = (int)(piece - (long long)cum[e] * slices);
+    slice = slices > 1 ? within / tiles : 0;
+    within -= slice * tiles;
+    tile = cum[e] + within;
     n_idx = within / m_tiles;
     row0 = first[e] + (within - n_idx * m_tiles) * tile_rows;
     row_end = end[e];
-    return true;
+    kb0 = slice * per, kb1 = min(k_blocks, kb0 + per);
   }
 };
+
+// Slices of a tile meet here.  A slab holds the accumulators of one piece, 16 bytes per lane side by side.
+struct I8Slices {
+  uint32_t* arrivals;       // [tiles][8 epilogue warps], zero at the start and at the end
+  int4* slabs;              // nullptr: no tile is cut
+};
+// N accumulators of every lane, at vector `at` of the warp's part of the slab
+template <int N>
+__device__ __forceinline__ void slab_store(int4* part, int at, int lane, const uint32_t* a) {
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i)
+    __stcg(part + (at + i) * 32 + lane, make_int4((int)a[4 * i], (int)a[4 * i + 1], (int)a[4 * i + 2], (int)a[4 * i + 3]));
+}
+// adds the other slices' accumulators; `stride`: vectors from one slice's slab to the next.  Up to 64 values are requested at once.
+template <int N>
+__device__ __forceinline__ void slab_add(const int4* part0, size_t stride, int slices, int mine, int at, int lane, uint32_t* a) {
+  constexpr int AT_ONCE = 64 / N;
+#pragma unroll 1
+  for (int s0 = 0; s0 < slices; s0 += AT_ONCE) {
+    int4 v[AT_ONCE][N / 4];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i)
+        v[j][i] = s0 + j < slices && s0 + j != mine ? __ldcg(part0 + (size_t)(s0 + j) * stride + (at + i) * 32 + lane) : make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        a[4 * i] += (uint32_t)v[j][i].x, a[4 * i + 1] += (uint32_t)v[j][i].y;
+        a[4 * i + 2] += (uint32_t)v[j][i].z, a[4 * i + 3] += (uint32_t)v[j][i].w;
+      }
+  }
+}
+// The warp's accumulators are in the slab: whether all other slices' are, too.
+__device__ __forceinline__ bool last_slice(uint32_t* counter, int slices, int lane) {
+  __syncwarp();
+  unsigned arrived = 0;
+  if (lane == 0) {
+    __threadfence();
+    arrived = atomicAdd(counter, 1u);
+    __threadfence();
+  }
+  const bool last = __shfl_sync(0xffffffffu, arrived, 0) == (unsigned)slices - 1;
+  __syncwarp();                                   // (orders the other lanes' reads behind lane 0's fence)
+  if (last && lane == 0) *counter = 0;            // for the next product with this scratch
+  return last;
+}
 
 // ---- output types: how many make 16 bytes, and the packing ----
 template <class T> struct Out;
@@ -144,22 +225,27 @@ __device__ __forceinline__ void zero_tail_rows(const I8Params& p, int part, int 
   for (size_t i = part; i < n; i += parts) at[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
+constexpr int L_MAX_PIECES = 320;                                             // where tiles are cut: a slab for each
+constexpr int L_PART = BN / 2 * 32 / 4;                                       // vectors of one epilogue warp's part of a slab
+constexpr size_t L_SLAB = (size_t)EPI_WARPS * L_PART * sizeof(int4);          // 128 KiB
+
 template <bool SWIGLU, class T>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b0,
-                 const __grid_constant__ CUtensorMap map_b1, const I8Params p) {
+                 const __grid_constant__ CUtensorMap map_b1, const I8Params p, const I8Slices sl) {
   chain_wait();
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_first[kMaxGroups], s_end[kMaxGroups], s_cum[kMaxGroups + 1];
   __shared__ __align__(16) float s_scale[EPI_WARPS][BN / 2];      // each epilogue warp's channel scales of its tile
   __shared__ uint32_t s_tmem_base;
-  __shared__ int s_abort;
+  __shared__ int s_abort, s_per;
 
   const uint32_t tiles_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bars = tiles_base + STAGES * STAGE_BYTES;
   const uint32_t bar_full = bars, bar_empty = bars + 8 * STAGES;
   const uint32_t bar_tfull = bars + 16 * STAGES, bar_tempty = bar_tfull + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k_blocks = (p.Kdim + BK - 1) / BK;
   volatile int* abort_flag = &s_abort;
 
   if (threadIdx.x == 0) {
@@ -169,31 +255,37 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tile_table<I8_THREADS>(p, BM, p.n_tiles, s_first, s_end, s_cum);
+  if (warp == 0) {
+    __syncwarp();
+    const int per = sl.slabs == nullptr ? k_blocks : blocks_per_slice(s_cum[p.E], k_blocks, gridDim.x, L_MAX_PIECES, 3000, 2200);
+    if (lane == 0) s_per = per;
+  }
   if (warp == 1) tmem_alloc(smem_u32(&s_tmem_base), TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
-  const int total_tiles = s_cum[p.E], k_blocks = (p.Kdim + BK - 1) / BK;
-  I8Cursor cur{s_first, s_end, s_cum, p.E, BM, 0};
+  I8Pieces q(s_first, s_end, s_cum, p.E, BM, k_blocks, s_per);
 
+  // PLAIN: the last tile of a row may have one weight box of channels only; then the other is neither loaded nor multiplied
+  auto one_box = [&]() { return !SWIGLU && q.n_idx * BN + BN_HALF >= p.N; };
   if (warp == 0) {
     // ===================== TMA producer =====================
     if (lane == 0) {
       uint32_t stage = 0, phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-        int row0, row_end, n_idx;
-        if (!cur.locate(tile, row0, row_end, n_idx)) break;
-        const int n0 = n_idx * (SWIGLU ? BN_HALF : BN);
-        for (int kb = 0; kb < k_blocks; ++kb) {
+      for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x) {
+        q.locate(piece);
+        const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN);
+        const bool one = one_box();
+        for (int kb = q.kb0; kb < q.kb1; ++kb) {
           if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status))) break;
           const uint32_t sa = tiles_base + stage * STAGE_BYTES, full = bar_full + 8 * stage;
-          mbar_expect_tx(full, STAGE_BYTES);
-          tma_load_2d(sa, &map_a, full, kb * BK, row0);
-          tma_load_3d(sa + A_BYTES, &map_b0, full, n0, kb * BK, cur.e);
-          if (SWIGLU) tma_load_3d(sa + A_BYTES + B_HALF_BYTES, &map_b1, full, n0, kb * BK, cur.e);
-          else        tma_load_3d(sa + A_BYTES + B_HALF_BYTES, &map_b0, full, n0 + BN_HALF, kb * BK, cur.e);
+          mbar_expect_tx(full, one ? STAGE_BYTES - B_HALF_BYTES : STAGE_BYTES);
+          tma_load_2d(sa, &map_a, full, kb * BK, q.row0);
+          tma_load_3d(sa + A_BYTES, &map_b0, full, n0, kb * BK, q.e);
+          if (SWIGLU)    tma_load_3d(sa + A_BYTES + B_HALF_BYTES, &map_b1, full, n0, kb * BK, q.e);
+          else if (!one) tma_load_3d(sa + A_BYTES + B_HALF_BYTES, &map_b0, full, n0 + BN_HALF, kb * BK, q.e);
           if (++stage == STAGES) stage = 0, phase ^= 1u;
         }
       }
@@ -203,18 +295,19 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     if (lane == 0) {
       uint32_t stage = 0, phase = 0, local = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x, ++local) {
-        const uint32_t buf = local & 1u, use = local >> 1;
+      for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x, ++local) {
+        q.locate(piece);
+        const uint32_t buf = local & 1u, use = local >> 1, desc = one_box() ? IDESC_I8_HALF : IDESC_I8;
         if (!(ok = mbar_wait(bar_tempty + 8 * buf, (use & 1u) ^ 1u, abort_flag, p.status))) break;
         tc_fence_after();
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = q.kb0; kb < q.kb1; ++kb) {
           if (!(ok = mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status))) break;
           tc_fence_after();
           const uint32_t sa = tiles_base + stage * STAGE_BYTES;
           const uint64_t da = desc_kmajor(sa), db = desc_nmajor(sa + A_BYTES);
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)     // A: +32 bytes along K inside the swizzle atom; B: +32 K rows = 4096 bytes
-            mma_i8(tmem_base + buf * BN, da + (uint64_t)(k * 2), db + (uint64_t)(k * 256), IDESC_I8, (kb | k) ? 1u : 0u);
+            mma_i8(tmem_base + buf * BN, da + (uint64_t)(k * 2), db + (uint64_t)(k * 256), desc, kb > q.kb0 || k > 0 ? 1u : 0u);
           mma_commit(bar_empty + 8 * stage);
           if (++stage == STAGES) stage = 0, phase ^= 1u;
         }
@@ -227,17 +320,16 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     float* my_scale = s_scale[warp - 2];
     uint32_t local = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x, ++local) {
-      int row0, row_end, n_idx;
-      if (!cur.locate(tile, row0, row_end, n_idx)) break;
+    for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x, ++local) {
+      q.locate(piece);
       const uint32_t buf = local & 1u, use = local >> 1;
-      const int row = row0 + quarter * 32 + lane;
-      const bool row_ok = row < row_end;
+      const int row = q.row0 + quarter * 32 + lane;
+      const bool row_ok = row < q.row_end;
       const float rs = row_ok ? p.row_scale[row] : 0.f;
       // channel scales of this warp's columns (SWIGLU: 64 of the gate, then 64 of the up product), zero past N
-      const int n0 = n_idx * (SWIGLU ? BN_HALF : BN) + half * (SWIGLU ? BN_HALF / 2 : BN_HALF);
+      const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN) + half * (SWIGLU ? BN_HALF / 2 : BN_HALF);
       {
-        const float* s = (SWIGLU && lane >= 16 ? p.scale1 : p.scale0) + (size_t)cur.e * p.N;
+        const float* s = (SWIGLU && lane >= 16 ? p.scale1 : p.scale0) + (size_t)q.e * p.N;
         const int n = n0 + (SWIGLU ? (lane & 15) : lane) * 4;
         __syncwarp();                            // the tile before has read its scales
         // (N is a multiple of 16, scales of 16-byte alignment: four at a time)
@@ -249,21 +341,45 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * BN;
+      constexpr int PER = Out<T>::kPer16, COLS = SWIGLU ? BN_HALF / 2 : BN_HALF;       // columns of this warp
+      const bool work = n0 < p.N;                                // (the second half of a tile may lie past N)
+      bool complete = work;
+      const int4* part0 = nullptr;                               // this warp's part of slice 0's slab
+      if (q.slices > 1 && work) {
+        part0 = sl.slabs + ((size_t)q.tile * q.slices * EPI_WARPS + (warp - 2)) * L_PART;
+        int4* part = const_cast<int4*>(part0) + (size_t)q.slice * EPI_WARPS * L_PART;
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += 32) {
+          uint32_t a[32];
+          tmem_ld32(t_row + half * COLS + c, a);
+          tmem_ld_wait();
+          slab_store<32>(part, c / 4, lane, a);
+          if constexpr (SWIGLU) {
+            tmem_ld32(t_row + BN_HALF + half * COLS + c, a);
+            tmem_ld_wait();
+            slab_store<32>(part, (COLS + c) / 4, lane, a);
+          }
+        }
+        complete = last_slice(sl.arrivals + q.tile * EPI_WARPS + (warp - 2), q.slices, lane);
+      }
       const unsigned ok_rows = __ballot_sync(0xffffffffu, row_ok);
       unsigned long long row_ptr[8];
       group8_row_pointers(static_cast<T*>(p.out) + (size_t)row * p.N, lane, row_ptr);
-      constexpr int PER = Out<T>::kPer16, COLS = SWIGLU ? BN_HALF / 2 : BN_HALF;       // columns of this warp
       // eight 16-byte pieces per lane at a time, exchanged so that a store writes 128 contiguous bytes of four rows
 #pragma unroll 1
-      for (int c0 = 0; c0 < COLS; c0 += 8 * PER) {
+      for (int c0 = 0; complete && c0 < COLS; c0 += 8 * PER) {
         uint4 v[8];
 #pragma unroll
         for (int part = 0; part < 8 * PER / 32; ++part) {
           const int c = c0 + part * 32;
-          uint32_t a[32], u[SWIGLU ? 32 : 1];
+          uint32_t a[32], u[SWIGLU ? 32 : 4];
           tmem_ld32(t_row + half * COLS + c, a);
           if constexpr (SWIGLU) tmem_ld32(t_row + BN_HALF + half * COLS + c, u);
           tmem_ld_wait();
+          if (q.slices > 1) {
+            slab_add<32>(part0, (size_t)EPI_WARPS * L_PART, q.slices, q.slice, c / 4, lane, a);
+            if constexpr (SWIGLU) slab_add<32>(part0, (size_t)EPI_WARPS * L_PART, q.slices, q.slice, (COLS + c) / 4, lane, u);
+          }
 #pragma unroll
           for (int j = 0; j < 32 / PER; ++j) {
             float f[PER];
@@ -302,26 +418,252 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
 }
 
+// ---------------------------------------------------------------- few rows per expert
+// Few rows per expert (decode): bound by the weights' bytes.  The weight tile takes the M side of the MMA and the rows the N
+// side, D^T[128 channels (tensor-memory lanes), 32 rows (columns)]: a stage is 32 KiB of weights and 4 KiB of rows, and six of
+// them are in flight.  Two epilogue warps per lane quarter, 16 of the rows each; a thread owns a channel of either weight tile.
+constexpr int S_NT = 32;                                     // rows per tile
+constexpr int S_THREADS = 64 + 32 * EPI_WARPS;
+constexpr int S_STAGES = 6;
+constexpr int S_W_BYTES = 2 * B_HALF_BYTES;
+constexpr int S_STAGE_BYTES = S_W_BYTES + S_NT * BK;         // 36 KiB
+constexpr int S_SMEM_BYTES = S_STAGES * S_STAGE_BYTES + 1024 /*alignment slack*/ + 512 /*barriers*/;
+constexpr int S_BUF_COLS = 2 * S_NT;
+constexpr int S_NBUF = TMEM_COLS / S_BUF_COLS;               // tiles in flight in tensor memory
+constexpr int S_MAX_PIECES = 640;                            // where tiles are cut: a slab for each
+constexpr int S_PART = 2 * (S_NT / 2) * 32 / 4;              // vectors of one epilogue warp's part of a slab
+constexpr size_t S_SLAB = (size_t)EPI_WARPS * S_PART * sizeof(int4);        // 32 KiB
+// D = int32, A = B = signed 8-bit, A MN-major (the weight tile), B K-major (the rows), N = 32, M = 128
+constexpr uint32_t IDESC_I8_SMALL = (2u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | ((uint32_t)(S_NT >> 3) << 17) |
+                                    ((uint32_t)(BM >> 4) << 24);
+
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld8(taddr, r); }
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+
 template <bool SWIGLU, class T>
-int run_large(const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1, const I8Params& p, cudaStream_t st) {
-  static unsigned char smem_set[64] = {0};
-  BWMOE_CUDA_OK(ensure_dynamic_smem(int8_gemm_kernel<SWIGLU, T>, SMEM_BYTES, smem_set));
-  const long long max_tiles = (long long)(ceil_div(p.M, BM) + p.E) * p.n_tiles;
-  const int grid = (int)std::min<long long>(gemm_sm_budget(), max_tiles);
-  BWMOE_CUDA_OK(launch_chained(int8_gemm_kernel<SWIGLU, T>, dim3(grid), dim3(I8_THREADS), SMEM_BYTES, st, ma, mb0, mb1, p));
+__global__ void __launch_bounds__(S_THREADS, 1)
+int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w0,
+                       const __grid_constant__ CUtensorMap map_w1, const I8Params p, const I8Slices sl) {
+  chain_wait();
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int s_first[kMaxGroups], s_end[kMaxGroups], s_cum[kMaxGroups + 1];
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort, s_per;
+
+  const uint32_t tiles_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = tiles_base + S_STAGES * S_STAGE_BYTES;
+  const uint32_t bar_full = bars, bar_empty = bars + 8 * S_STAGES;
+  const uint32_t bar_tfull = bars + 16 * S_STAGES, bar_tempty = bar_tfull + 8 * S_NBUF;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k_blocks = (p.Kdim + BK - 1) / BK;
+  volatile int* abort_flag = &s_abort;
+
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int s = 0; s < S_STAGES; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 1);
+    for (int b = 0; b < S_NBUF; ++b) mbar_init(bar_tfull + 8 * b, 1), mbar_init(bar_tempty + 8 * b, EPI_WARPS);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tile_table<S_THREADS>(p, S_NT, p.n_tiles, s_first, s_end, s_cum);
+  if (warp == 0) {
+    __syncwarp();
+    const int per = blocks_per_slice(s_cum[p.E], k_blocks, gridDim.x, S_MAX_PIECES, 1500, 100);
+    if (lane == 0) s_per = per;
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&s_tmem_base), TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = s_tmem_base;
+  I8Pieces q(s_first, s_end, s_cum, p.E, S_NT, k_blocks, s_per);
+
+  if (warp == 0) {
+    // ===================== TMA producer =====================
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x) {
+        q.locate(piece);
+        const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN);
+        for (int kb = q.kb0; kb < q.kb1; ++kb) {
+          if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status))) break;
+          const uint32_t sw = tiles_base + stage * S_STAGE_BYTES, full = bar_full + 8 * stage;
+          mbar_expect_tx(full, S_STAGE_BYTES);
+          tma_load_3d(sw, &map_w0, full, n0, kb * BK, q.e);
+          if (SWIGLU) tma_load_3d(sw + B_HALF_BYTES, &map_w1, full, n0, kb * BK, q.e);
+          else        tma_load_3d(sw + B_HALF_BYTES, &map_w0, full, n0 + BN_HALF, kb * BK, q.e);
+          tma_load_2d(sw + S_W_BYTES, &map_x, full, kb * BK, q.row0);
+          if (++stage == S_STAGES) stage = 0, phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ===================== MMA issuer =====================
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, it = 0;
+      bool ok = true;
+      for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x, ++it) {
+        q.locate(piece);
+        const uint32_t buf = it % S_NBUF, use = it / S_NBUF;
+        if (!(ok = mbar_wait(bar_tempty + 8 * buf, (use & 1u) ^ 1u, abort_flag, p.status))) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + buf * S_BUF_COLS;
+        for (int kb = q.kb0; kb < q.kb1; ++kb) {
+          if (!(ok = mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status))) break;
+          tc_fence_after();
+          const uint32_t sw = tiles_base + stage * S_STAGE_BYTES;
+          const uint64_t db = desc_kmajor(sw + S_W_BYTES), da0 = desc_nmajor(sw), da1 = desc_nmajor(sw + B_HALF_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k) {     // weights: +32 K rows = 4096 bytes; rows: +32 bytes along K
+            mma_i8(d, da0 + (uint64_t)(k * 256), db + (uint64_t)(k * 2), IDESC_I8_SMALL, kb > q.kb0 || k > 0 ? 1u : 0u);
+            mma_i8(d + S_NT, da1 + (uint64_t)(k * 256), db + (uint64_t)(k * 2), IDESC_I8_SMALL, kb > q.kb0 || k > 0 ? 1u : 0u);
+          }
+          mma_commit(bar_empty + 8 * stage);
+          if (++stage == S_STAGES) stage = 0, phase ^= 1u;
+        }
+        if (ok) mma_commit(bar_tfull + 8 * buf);
+      }
+    }
+  } else {
+    // ===================== epilogue (warps 2..9) =====================
+    const int quarter = warp & 3, c0 = ((warp - 2) >> 2) * (S_NT / 2), f = quarter * 32 + lane;
+    uint32_t it = 0;
+    bool ok = true;
+    for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x, ++it) {
+      q.locate(piece);
+      const uint32_t buf = it % S_NBUF, use = it / S_NBUF;
+      const int n_valid = min(S_NT / 2, q.row_end - q.row0 - c0);       // this warp's rows; none: <= 0
+      const int n = q.n_idx * (SWIGLU ? BN_HALF : BN) + f, m = SWIGLU ? n : n + BN_HALF;      // the thread's two channels
+      const float s0 = n < p.N ? p.scale0[(size_t)q.e * p.N + n] : 0.f;
+      const float s1 = m < p.N ? (SWIGLU ? p.scale1 : p.scale0)[(size_t)q.e * p.N + m] : 0.f;
+      const float my_rs = lane < n_valid ? p.row_scale[q.row0 + c0 + lane] : 0.f;
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * buf, use & 1u, abort_flag, p.status));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * S_BUF_COLS + c0;
+      auto finish = [&](auto columns) {
+        constexpr int NC = decltype(columns)::value;
+        uint32_t a0[NC], a1[NC];
+        tmem_ld_cols(t_row, a0);
+        tmem_ld_cols(t_row + S_NT, a1);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
+        if (q.slices > 1) {
+          const int4* part0 = sl.slabs + ((size_t)q.tile * q.slices * EPI_WARPS + (warp - 2)) * S_PART;
+          int4* part = const_cast<int4*>(part0) + (size_t)q.slice * EPI_WARPS * S_PART;
+          slab_store<NC>(part, 0, lane, a0);
+          slab_store<NC>(part, S_NT / 8, lane, a1);
+          if (!last_slice(sl.arrivals + q.tile * EPI_WARPS + (warp - 2), q.slices, lane)) return;
+          slab_add<NC>(part0, (size_t)EPI_WARPS * S_PART, q.slices, q.slice, 0, lane, a0);
+          slab_add<NC>(part0, (size_t)EPI_WARPS * S_PART, q.slices, q.slice, S_NT / 8, lane, a1);
+        }
+        T* out = static_cast<T*>(p.out) + (size_t)(q.row0 + c0) * p.N;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float rs = __shfl_sync(0xffffffffu, my_rs, c);
+          const float v0 = __int2float_rn((int)a0[c]) * rs * s0, v1 = __int2float_rn((int)a1[c]) * rs * s1;
+          if (c >= n_valid) continue;
+          if (SWIGLU) {
+            if (n < p.N) out[(size_t)c * p.N + n] = Out<T>::one(swiglu<T>(v0, v1));
+          } else {
+            if (n < p.N) out[(size_t)c * p.N + n] = Out<T>::one(v0);
+            if (m < p.N) out[(size_t)c * p.N + m] = Out<T>::one(v1);
+          }
+        }
+      };
+      if (n_valid > 8) finish(std::integral_constant<int, 16>{});
+      else if (n_valid > 0) finish(std::integral_constant<int, 8>{});
+      else {                                            // the tile has no rows for this warp
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
+      }
+    }
+    zero_tail_rows<T>(p, blockIdx.x * (32 * EPI_WARPS) + threadIdx.x - 64, gridDim.x * (32 * EPI_WARPS));
+  }
+
+  if (*abort_flag) {            // copies that are still in flight land before the shared memory is released
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+}
+
+// rows [rows, kdim] of 8-bit integers: box 128 (K) x 32 (rows), 128-byte swizzle (kind 2: the map of the block-scale kernel's rows)
+int make_map_rows32(CUtensorMap* map, const void* base, int rows, int kdim) {
+  if (tensor_map_lookup(2, base, rows, kdim, 0, map)) return BWMOE_OK;
+  auto fn = encode_fn();
+  BWMOE_REQUIRE(fn != nullptr, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+  cuuint64_t dims[2] = {(cuuint64_t)kdim, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)kdim};
+  cuuint32_t box[2] = {BK, 32};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  BWMOE_REQUIRE(r == CUDA_SUCCESS, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled(rows=%d k=%d) failed: %d", rows, kdim, (int)r);
+  tensor_map_store(2, base, rows, kdim, 0, *map);
   return BWMOE_OK;
 }
 
-template <bool SWIGLU>
-int run_typed(const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1, const I8Params& p, int dtype, cudaStream_t st) {
-  if (dtype == BWMOE_F32) return run_large<SWIGLU, float>(ma, mb0, mb1, p, st);
-  if (dtype == BWMOE_F16) return run_large<SWIGLU, __half>(ma, mb0, mb1, p, st);
-  return run_large<SWIGLU, __nv_bfloat16>(ma, mb0, mb1, p, st);
+// Which kernel a product gets.  32-row tiles: few rows per expert, or tiles so few that they fit the SMs at once (and K blocks
+// few enough that reading the weights again for every 32 rows does not count).  Measured, us, 32-row tiles against 128-row tiles
+// (launched one after the other, weights from memory):
+//   8 experts of 4096 x 14336 (SwiGLU):  1 row each 144 / 203,  32 rows 150 / 158,  48 rows 161 / 158,  128 rows 300 / 167
+//   64 experts of 2048 x 1408:           8 rows each 35.6 / 40.6,  32 rows 37.2 / 38.6,  48 rows 43.8 / 39.4
+//   one matrix 4096 x 14336:  1 row 17.4 / 24.5,  48 rows 17.7 / 23.1,  128 rows 29.0 / 23.4
+//   one matrix 2048 x 2048:  512 rows 11.7 / 13.2;   14336 x 4096:  48 rows 22.5 / 32.5,  128 rows 28.5 / 32.9,  256 rows 44.6 / 32.3
+bool small_applies(int M, int K, int n_tiles, int E) {
+  if (M <= 32ll * E) return true;
+  const long long tiles = ((long long)M / S_NT + E) * n_tiles;
+  return tiles <= sm_count() && tiles * ceil_div(K, BK) <= 8192;
+}
+// Whether the other kernel's tiles may leave SMs without work, so that slabs are worth their memory.
+bool may_slice(int M, int n_tiles) { return (long long)ceil_div(M, BM) * n_tiles < sm_count(); }
+
+// Scratch: the status word, the counters (tiles that are cut have two slices at least), the slabs.
+constexpr size_t kArrivalsAt = 16;
+constexpr size_t kSlabsAt = kArrivalsAt + (S_MAX_PIECES > L_MAX_PIECES ? S_MAX_PIECES : L_MAX_PIECES) / 2 * EPI_WARPS * sizeof(uint32_t);
+
+template <class Kernel>
+int run(Kernel kernel, bool small, const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1, const I8Params& p,
+        const I8Slices& sl, unsigned char (&smem_set)[64], cudaStream_t st) {
+  const int smem = small ? S_SMEM_BYTES : SMEM_BYTES, k_blocks = ceil_div(p.Kdim, BK);
+  BWMOE_CUDA_OK(ensure_dynamic_smem(kernel, smem, smem_set));
+  const long long max_pieces = (long long)(ceil_div(p.M, small ? S_NT : BM) + p.E) * p.n_tiles * (sl.slabs ? k_blocks : 1);
+  const int grid = (int)std::min<long long>(gemm_sm_budget(), max_pieces);
+  BWMOE_CUDA_OK(launch_chained(kernel, dim3(grid), dim3(small ? S_THREADS : I8_THREADS), smem, st, ma, mb0, mb1, p, sl));
+  return BWMOE_OK;
+}
+template <bool SWIGLU, class T>
+int run_typed(bool small, const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1, const I8Params& p,
+              const I8Slices& sl, cudaStream_t st) {
+  static unsigned char smem_set[2][64] = {};
+  return small ? run(int8_gemm_small_kernel<SWIGLU, T>, true, ma, mb0, mb1, p, sl, smem_set[1], st)
+               : run(int8_gemm_kernel<SWIGLU, T>, false, ma, mb0, mb1, p, sl, smem_set[0], st);
+}
+
+// fn(type tag)
+template <class F>
+int for_type(int dtype, F fn) {
+  if (dtype == BWMOE_F32) return fn(TypeTag<float>{});
+  if (dtype == BWMOE_F16) return fn(TypeTag<__half>{});
+  return fn(TypeTag<__nv_bfloat16>{});
 }
 
 }  // namespace
 
-size_t int8_scratch_bytes(int /*M*/, int /*K*/, int /*N*/, int /*E*/) { return 256; }
+size_t int8_clear_bytes() { return kSlabsAt; }
+size_t int8_scratch_bytes(int M, int K, int N, int E) {
+  // for one product and for SwiGLU, which has more tiles
+  size_t slabs = 0;
+  for (const int n_tiles : {ceil_div(N, BN), ceil_div(N, BN_HALF)})
+    slabs = std::max(slabs, small_applies(M, K, n_tiles, E) ? S_MAX_PIECES * S_SLAB : may_slice(M, n_tiles) ? L_MAX_PIECES * L_SLAB : 0);
+  return kSlabsAt + slabs;
+}
 
 int check_int8_gemm(const void* a, const float* row_scale, const int32_t* offsets, const void* w0, const void* w1,
                     const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, const void* out,
@@ -342,18 +684,26 @@ int check_int8_gemm(const void* a, const float* row_scale, const int32_t* offset
 }
 
 int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offsets, const void* w0, const void* w1,
-                     const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, void* out, int32_t* status,
-                     cudaStream_t st, bool clear_status) {
+                     const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, void* out, void* scratch,
+                     cudaStream_t st, bool clear, int32_t* status) {
   const bool swiglu = w1 != nullptr;
+  if (status == nullptr) status = static_cast<int32_t*>(scratch);
   if (int rc = check_int8_gemm(a, row_scale, offsets, w0, w1, scale0, scale1, M, K, N, E, dtype, out, status)) return rc;
-  if (clear_status) BWMOE_CUDA_OK(cudaMemsetAsync(status, 0, 16, st));
+  if (clear) BWMOE_CUDA_OK(cudaMemsetAsync(scratch, 0, kSlabsAt, st));
   const int n_tiles = ceil_div(N, swiglu ? BN_HALF : BN);
+  const bool small = small_applies(M, K, n_tiles, E);
   CUtensorMap ma, mb0, mb1;
-  if (int rc = make_map_a(&ma, a, M, K)) return rc;
+  if (int rc = small ? make_map_rows32(&ma, a, M, K) : make_map_a(&ma, a, M, K)) return rc;
   if (int rc = make_map_b(&mb0, w0, E, K, N)) return rc;
   if (int rc = make_map_b(&mb1, swiglu ? w1 : w0, E, K, N)) return rc;
   const I8Params p{offsets, row_scale, scale0, scale1, out, status, E, M, K, N, n_tiles};
-  return swiglu ? run_typed<true>(ma, mb0, mb1, p, dtype, st) : run_typed<false>(ma, mb0, mb1, p, dtype, st);
+  uint8_t* s = static_cast<uint8_t*>(scratch);
+  const bool slabs = small || may_slice(M, n_tiles);
+  const I8Slices sl{reinterpret_cast<uint32_t*>(s + kArrivalsAt), slabs ? reinterpret_cast<int4*>(s + kSlabsAt) : nullptr};
+  return for_type(dtype, [&](auto tag) {
+    using T = typename decltype(tag)::type;
+    return swiglu ? run_typed<true, T>(small, ma, mb0, mb1, p, sl, st) : run_typed<false, T>(small, ma, mb0, mb1, p, sl, st);
+  });
 }
 
 }  // namespace bwmoe

@@ -1,9 +1,18 @@
 // Activations -> 8-bit integers, one scale per row:
 //   scale = fl32(max|x| / 127)      code = x / scale rounded to the nearest whole number, ties to even
-// The scale is rounded to fp32 once and the codes are exact for that scale: a product with the reciprocal may end on the
-// wrong side of a border n + 1/2, so quotients that come near one are decided by the sign of x - (n + 1/2) * scale, which
-// one fused multiply-add gives exactly.  A row of zeros has scale 0 and codes 0.  A row with an infinity or a NaN has no
-// representation in 8 bits: its scale is NaN and its codes are 0, so that every product of the row is NaN.
+// The scale is rounded to fp32 once and the codes are exact for that scale.  A row of zeros has scale 0 and codes 0.  A row
+// with an infinity or a NaN has no representation in 8 bits: its scale is NaN and its codes are 0, so that every product of
+// the row is NaN.
+//
+// A product with the reciprocal may end on the wrong side of a border n + 1/2.  For 16-bit inputs that is settled per row:
+// with p significant bits (8 or 11) the quotient 127 x / max|x| of two such numbers is either on a border or at least
+// 2^-(p+9) of its value away from every border, and scale = max|x| / 127 * (1 + d), |d| <= 2^-24, moves the quotients on a
+// border all to the same side, the one that the sign of d gives.  So the reciprocal is made 2^-21 smaller (d > 0) or larger
+// (d < 0): more than its own roundings and d together (2^-22), and less than 2^-20.  With d = 0 borders are ties; they come
+// out right where the reciprocal is exact, and the other rows (one in 100 in fp16) are divided one by one.  (16-bit inputs
+// meet borders once in 500 values: with each checked and decided by itself 368 us for 32768 rows of 14336, 196 us for 16384
+// x 4096 into two rows each.)  For fp32 inputs a piece with a quotient within 1e-5 of a border (one in 3000) is decided by
+// the sign of x - (n + 1/2) * scale, which one fused multiply-add gives exactly.
 //
 // Bound by memory: a row is read once - each thread keeps its pieces of 16 elements in registers between the maximum and
 // the codes - and written to all of the rows it is needed in (the K rows of its token, or one).  The conversion adds
@@ -18,8 +27,8 @@ constexpr int kThreads = 256;
 constexpr int kKept = 4;                       // pieces of a row that a thread keeps in registers
 constexpr float kTinyScale = 7.888609052210118e-31f;     // 2^-100: below it products with the scale may lose bits
 
-// |x| / scale, rounded exactly (ties to even); scale > 0
-__device__ int exact_code(float x, float scale) {
+// x / scale, rounded exactly (ties to even); scale > 0
+__device__ __noinline__ int exact_code(float x, float scale) {
   const float a = fabsf(x), f = floorf(fminf(__fdiv_rn(a, scale), 127.f));
   // the sign of a - (f + 1/2) * scale; doubled where the scale's last bits are the smallest there are
   const float r = scale >= kTinyScale ? fmaf(-(f + 0.5f), scale, a) : fmaf(-(2.f * f + 1.f), scale, 2.f * a);
@@ -92,9 +101,42 @@ __device__ __forceinline__ float bits_value(uint32_t m, float) { return __uint_a
 __device__ __forceinline__ float bits_value(uint32_t m, __half) { return __half2float(__ushort_as_half((unsigned short)m)); }
 __device__ __forceinline__ float bits_value(uint32_t m, __nv_bfloat16) { return __uint_as_float(m << 16); }
 
-// scale >= kTinyScale and finite
+__device__ __forceinline__ uint4 pack_codes(const uint32_t (&b)[16]) {      // the low bytes
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// How a row's codes are formed.
+struct RowScale {
+  float scale, inv;
+  bool none;          // zeros, or a row without a representation: all codes 0
+  bool one_by_one;    // every quotient by itself
+};
 template <class T>
-__device__ __forceinline__ uint4 piece_codes(const Piece16<T>& p, float scale, float inv) {
+__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
+  const float amax = bits_value(amax_bits, T{});
+  RowScale r;
+  const bool finite = amax <= 3.402823466e38f;
+  r.scale = finite ? __fdiv_rn(amax, 127.f) : __uint_as_float(0x7fc00000u);
+  r.none = !(r.scale > 0.f);
+  r.inv = __fdiv_rn(1.f, r.scale);
+  r.one_by_one = r.scale < kTinyScale;
+  if (sizeof(T) == 2) {
+    const float d = fmaf(r.scale, 127.f, -amax);      // (its sign is exact)
+    constexpr float kBias = 4.76837158203125e-7f;     // 2^-21
+    if (d > 0.f) r.inv *= 1.f - kBias;
+    if (d < 0.f) r.inv *= 1.f + kBias;
+    if (d == 0.f && (__float_as_uint(r.scale) & 0x7fffffu) != 0u) r.one_by_one = true;
+  }
+  return r;
+}
+
+template <class T>
+__device__ __forceinline__ uint4 piece_codes(const Piece16<T>& p, const RowScale& r) {
+  if (r.none) return make_uint4(0u, 0u, 0u, 0u);
   constexpr float kMagic = 12582912.f;          // 1.5 * 2^23: the sum's last bit is worth 1
   float f[16];
   p.values(f);
@@ -102,25 +144,16 @@ __device__ __forceinline__ uint4 piece_codes(const Piece16<T>& p, float scale, f
   float far = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float m = fmaf(f[i], inv, kMagic);
-    far = fmaxf(far, fabsf(fmaf(f[i], inv, kMagic - m)));
+    const float m = fmaf(f[i], r.inv, kMagic);
+    if (sizeof(T) == 4) far = fmaxf(far, fabsf(fmaf(f[i], r.inv, kMagic - m)));
     b[i] = __float_as_uint(m);
   }
-  // f * inv is off by at most 127 * 2^-24 = 7.6e-6 (the reciprocal's rounding), its distance from the code by 2^-25 more;
-  // anything nearer to a border is decided exactly: one piece in 3000, one warp in 100
-  if (far > 0.49999f) {
-#pragma unroll 1
-    for (int i = 0; i < 16; ++i) {
+  // fp32: f * inv is off by at most 127 * 2^-24 = 7.6e-6 (the reciprocal's rounding), its distance from the code by 2^-25 more
+  if (r.one_by_one || (sizeof(T) == 4 && far > 0.49999f)) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j == i) b[j] = (uint32_t)exact_code(f[j], scale);
-    }
+    for (int i = 0; i < 16; ++i) b[i] = (uint32_t)exact_code(f[i], r.scale);
   }
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return pack_codes(b);
 }
 
 // wpr warps (1, 2, 4 or 8) share a row.  pos == nullptr: row t is written to row t.
@@ -160,32 +193,12 @@ quant_int8_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ pos,
     for (int i = 0; i < wpr; ++i) m = max(m, s_max[warp - sub + i]);
   }
   if (!live) return;
-  const float amax = bits_value(m, T{});
-  const bool finite = amax <= 3.402823466e38f;
-  const float scale = finite ? __fdiv_rn(amax, 127.f) : __uint_as_float(0x7fc00000u);
-  const float inv = __fdiv_rn(1.f, scale);
-  auto convert = [&](const Piece16<T>& q) {
-    if (scale >= kTinyScale) return piece_codes(q, scale, inv);
-    uint4 o = make_uint4(0u, 0u, 0u, 0u);       // zeros, and rows that have no representation
-    if (finite && scale > 0.f) {
-      float f[16];
-      q.values(f);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[i] |= ((uint32_t)exact_code(f[4 * i + j], scale) & 0xffu) << (8 * j);
-      }
-      o = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    return o;
-  };
+  const RowScale r = row_scale<T>(m);
   const int M = n_tok * K, n_rows = pos != nullptr ? offsets[E] : M;
   auto store = [&](int c, uint4 o) {
     if (pos == nullptr) {
       reinterpret_cast<uint4*>(codes + (size_t)t * D)[c] = o;
-      if (c == 0) scales[t] = scale;
+      if (c == 0) scales[t] = r.scale;
       return;
     }
 #pragma unroll 4
@@ -193,7 +206,7 @@ quant_int8_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ pos,
       const int s = t * K + k, p = pos[s];
       if ((unsigned)p < (unsigned)M) {          // a plan is data from outside the kernel
         reinterpret_cast<uint4*>(codes + (size_t)p * D)[c] = o;
-        if (c == 0) scales[p] = scale;
+        if (c == 0) scales[p] = r.scale;
       }
       if (s >= n_rows) {                        // a row that no slot owns
         reinterpret_cast<uint4*>(codes + (size_t)s * D)[c] = make_uint4(0u, 0u, 0u, 0u);
@@ -203,11 +216,11 @@ quant_int8_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ pos,
   };
 #pragma unroll
   for (int i = 0; i < kKept; ++i)
-    if (c0 + i * step < pieces) store(c0 + i * step, convert(kept[i]));
+    if (c0 + i * step < pieces) store(c0 + i * step, piece_codes(kept[i], r));
   for (int c = c0 + kKept * step; c < pieces; c += step) {
     Piece16<T> q;
     q.load(src + (size_t)c * 16);
-    store(c, convert(q));
+    store(c, piece_codes(q, r));
   }
 }
 
