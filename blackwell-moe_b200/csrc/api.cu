@@ -387,12 +387,12 @@ int run_int8_pipeline(const void* x, const float* weights, const int32_t* indice
     return rc;
   if ((rc = launch_quant_int8_rows(x, pos, offsets, T, D, E, K, dtype, at<void>(ws, L.xq), sx, st))) return rc;
   if ((rc = launch_int8_gemm(at<void>(ws, L.xq), sx, offsets, wg, wu, sg, su, M, D, H, E, dtype, at<void>(ws, L.h),
-                             at<void>(ws, L.gemm_scratch), st, false, status)))
+                             at<void>(ws, L.gemm_scratch), st, false, status, true)))
     return rc;
   if ((rc = launch_quant_int8_rows(at<void>(ws, L.h), nullptr, nullptr, M, H, 1, 1, dtype, at<void>(ws, L.hq), sh, st)))
     return rc;
   if ((rc = launch_int8_gemm(at<void>(ws, L.hq), sh, offsets, wd, nullptr, sd, nullptr, M, H, D, E, dtype, at<void>(ws, L.y),
-                             at<void>(ws, L.gemm_scratch), st, false, status)))
+                             at<void>(ws, L.gemm_scratch), st, false, status, true)))
     return rc;
   return launch_unpermute_rows(at<void>(ws, L.y), pos, weights, T, D, K, dtype, out, st);
 }
@@ -954,7 +954,7 @@ int bwmoe_int_matmul(const void* x, const void* w, const float* scale, int T, in
                                       int8_clear_bytes()))
     return rc;
   return launch_int8_gemm(at<void>(ws, codes), at<float>(ws, scales), nullptr, w, nullptr, scale, nullptr, T, K, N, 1, dtype, out,
-                          ws, st);
+                          ws, st, false, nullptr, true);
 }
 
 size_t bwmoe_workspace_bytes_int(int T, int D, int H, int E, int K) {

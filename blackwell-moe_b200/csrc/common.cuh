@@ -38,7 +38,7 @@ inline cudaStream_t counted(cudaStream_t st) {
 // kernel call it: a kernel that ends without it could end before the one in front, and the kernel behind it would then
 // start too early.  A kernel that calls it may also be launched the ordinary way (the instruction returns at once).
 // Before the wait a kernel may touch only what the kernel in front neither writes nor, where it is written here, reads
-// (two do: plan_quant_kernel requests x, transpose_gate_kernel does all of its work).  That is sound because everything
+// (plan_quant_kernel requests x, transpose_gate_kernel does all of its work, the 8-bit integer products request weights).  That is sound because everything
 // BEFORE the kernel in front is complete by then, which in turn rests on every kernel of the chain waiting before it
 // lets the next one be scheduled - by ending, or by chain_next().
 //
@@ -307,7 +307,9 @@ int check_int8_gemm(const void* a, const float* row_scale, const int32_t* offset
                     const int32_t* status);
 int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offsets, const void* w0, const void* w1,
                      const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, void* out, void* scratch,
-                     cudaStream_t st, bool clear = false, int32_t* status = nullptr);
+                     cudaStream_t st, bool clear = false, int32_t* status = nullptr, bool early = false);
+// early: the kernel in front in the stream is launch_quant_int8_rows() of `a`, and nothing else that the product reads is
+// written by it.
 
 // Monotone map of a float onto unsigned integers (a < b  <=>  key(a) < key(b); -0 is folded onto +0 first).
 __device__ __forceinline__ unsigned order_key(float v) {

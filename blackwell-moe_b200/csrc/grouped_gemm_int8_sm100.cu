@@ -55,6 +55,9 @@ struct I8Params {
   void* out;                // [M, N]
   int32_t* status;
   int E, M, Kdim, N, n_tiles;
+  // The kernel in front is the one that quantised the rows, and it lets this one be scheduled beside it: weights, scales and
+  // offsets are older than that kernel, so set-up and the first weight tiles do not wait for it.
+  bool early;
 };
 
 // Segment e, clamped to the rows there are: offsets are data from outside the kernel.
@@ -129,6 +132,17 @@ struct I8Pieces {
     kb0 = slice * per, kb1 = min(k_blocks, kb0 + per);
   }
 };
+
+// The weights of the CTA's first stages (all stages are free then); the number of stages begun.
+template <class Load>
+__device__ __forceinline__ int first_weights(I8Pieces q, int stages, Load load_weights) {
+  int n = 0;
+  for (long long piece = blockIdx.x; n < stages && piece < q.total; piece += gridDim.x) {
+    q.locate(piece);
+    for (int kb = q.kb0; n < stages && kb < q.kb1; ++kb, ++n) load_weights(q, kb, n);
+  }
+  return n;
+}
 
 // Slices of a tile meet here.  A slab holds the accumulators of one piece, 16 bytes per lane side by side.
 struct I8Slices {
@@ -233,7 +247,7 @@ template <bool SWIGLU, class T>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b0,
                  const __grid_constant__ CUtensorMap map_b1, const I8Params p, const I8Slices sl) {
-  chain_wait();
+  if (!p.early) chain_wait();
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_first[kMaxGroups], s_end[kMaxGroups], s_cum[kMaxGroups + 1];
   __shared__ __align__(16) float s_scale[EPI_WARPS][BN / 2];      // each epilogue warp's channel scales of its tile
@@ -268,7 +282,21 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   I8Pieces q(s_first, s_end, s_cum, p.E, BM, k_blocks, s_per);
 
   // PLAIN: the last tile of a row may have one weight box of channels only; then the other is neither loaded nor multiplied
-  auto one_box = [&]() { return !SWIGLU && q.n_idx * BN + BN_HALF >= p.N; };
+  auto one_box = [&](const I8Pieces& q) { return !SWIGLU && q.n_idx * BN + BN_HALF >= p.N; };
+  auto load_weights = [&](const I8Pieces& q, int kb, uint32_t stage) {
+    const uint32_t sb = tiles_base + stage * STAGE_BYTES + A_BYTES, full = bar_full + 8 * stage;
+    const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN);
+    const bool one = one_box(q);
+    mbar_expect_tx(full, one ? STAGE_BYTES - B_HALF_BYTES : STAGE_BYTES);
+    tma_load_3d(sb, &map_b0, full, n0, kb * BK, q.e);
+    if (SWIGLU)    tma_load_3d(sb + B_HALF_BYTES, &map_b1, full, n0, kb * BK, q.e);
+    else if (!one) tma_load_3d(sb + B_HALF_BYTES, &map_b0, full, n0 + BN_HALF, kb * BK, q.e);
+  };
+  int ahead = 0;                // stages whose weights are on their way already
+  if (p.early) {
+    if (threadIdx.x == 0) ahead = first_weights(q, STAGES, load_weights);
+    chain_wait();
+  }
   if (warp == 0) {
     // ===================== TMA producer =====================
     if (lane == 0) {
@@ -276,16 +304,14 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       bool ok = true;
       for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x) {
         q.locate(piece);
-        const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN);
-        const bool one = one_box();
         for (int kb = q.kb0; kb < q.kb1; ++kb) {
-          if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status))) break;
-          const uint32_t sa = tiles_base + stage * STAGE_BYTES, full = bar_full + 8 * stage;
-          mbar_expect_tx(full, one ? STAGE_BYTES - B_HALF_BYTES : STAGE_BYTES);
-          tma_load_2d(sa, &map_a, full, kb * BK, q.row0);
-          tma_load_3d(sa + A_BYTES, &map_b0, full, n0, kb * BK, q.e);
-          if (SWIGLU)    tma_load_3d(sa + A_BYTES + B_HALF_BYTES, &map_b1, full, n0, kb * BK, q.e);
-          else if (!one) tma_load_3d(sa + A_BYTES + B_HALF_BYTES, &map_b0, full, n0 + BN_HALF, kb * BK, q.e);
+          if (ahead > 0) {
+            --ahead;
+          } else {
+            if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status))) break;
+            load_weights(q, kb, stage);
+          }
+          tma_load_2d(tiles_base + stage * STAGE_BYTES, &map_a, bar_full + 8 * stage, kb * BK, q.row0);
           if (++stage == STAGES) stage = 0, phase ^= 1u;
         }
       }
@@ -297,7 +323,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       bool ok = true;
       for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x, ++local) {
         q.locate(piece);
-        const uint32_t buf = local & 1u, use = local >> 1, desc = one_box() ? IDESC_I8_HALF : IDESC_I8;
+        const uint32_t buf = local & 1u, use = local >> 1, desc = one_box(q) ? IDESC_I8_HALF : IDESC_I8;
         if (!(ok = mbar_wait(bar_tempty + 8 * buf, (use & 1u) ^ 1u, abort_flag, p.status))) break;
         tc_fence_after();
         for (int kb = q.kb0; kb < q.kb1; ++kb) {
@@ -444,7 +470,7 @@ template <bool SWIGLU, class T>
 __global__ void __launch_bounds__(S_THREADS, 1)
 int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w0,
                        const __grid_constant__ CUtensorMap map_w1, const I8Params p, const I8Slices sl) {
-  chain_wait();
+  if (!p.early) chain_wait();
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_first[kMaxGroups], s_end[kMaxGroups], s_cum[kMaxGroups + 1];
   __shared__ uint32_t s_tmem_base;
@@ -477,6 +503,19 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
   const uint32_t tmem_base = s_tmem_base;
   I8Pieces q(s_first, s_end, s_cum, p.E, S_NT, k_blocks, s_per);
 
+  auto load_weights = [&](const I8Pieces& q, int kb, uint32_t stage) {
+    const uint32_t sw = tiles_base + stage * S_STAGE_BYTES, full = bar_full + 8 * stage;
+    const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN);
+    mbar_expect_tx(full, S_STAGE_BYTES);
+    tma_load_3d(sw, &map_w0, full, n0, kb * BK, q.e);
+    if (SWIGLU) tma_load_3d(sw + B_HALF_BYTES, &map_w1, full, n0, kb * BK, q.e);
+    else        tma_load_3d(sw + B_HALF_BYTES, &map_w0, full, n0 + BN_HALF, kb * BK, q.e);
+  };
+  int ahead = 0;                // stages whose weights are on their way already
+  if (p.early) {
+    if (threadIdx.x == 0) ahead = first_weights(q, S_STAGES, load_weights);
+    chain_wait();
+  }
   if (warp == 0) {
     // ===================== TMA producer =====================
     if (lane == 0) {
@@ -484,15 +523,14 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       bool ok = true;
       for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x) {
         q.locate(piece);
-        const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN);
         for (int kb = q.kb0; kb < q.kb1; ++kb) {
-          if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status))) break;
-          const uint32_t sw = tiles_base + stage * S_STAGE_BYTES, full = bar_full + 8 * stage;
-          mbar_expect_tx(full, S_STAGE_BYTES);
-          tma_load_3d(sw, &map_w0, full, n0, kb * BK, q.e);
-          if (SWIGLU) tma_load_3d(sw + B_HALF_BYTES, &map_w1, full, n0, kb * BK, q.e);
-          else        tma_load_3d(sw + B_HALF_BYTES, &map_w0, full, n0 + BN_HALF, kb * BK, q.e);
-          tma_load_2d(sw + S_W_BYTES, &map_x, full, kb * BK, q.row0);
+          if (ahead > 0) {
+            --ahead;
+          } else {
+            if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status))) break;
+            load_weights(q, kb, stage);
+          }
+          tma_load_2d(tiles_base + stage * S_STAGE_BYTES + S_W_BYTES, &map_x, bar_full + 8 * stage, kb * BK, q.row0);
           if (++stage == S_STAGES) stage = 0, phase ^= 1u;
         }
       }
@@ -685,7 +723,7 @@ int check_int8_gemm(const void* a, const float* row_scale, const int32_t* offset
 
 int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offsets, const void* w0, const void* w1,
                      const float* scale0, const float* scale1, int M, int K, int N, int E, int dtype, void* out, void* scratch,
-                     cudaStream_t st, bool clear, int32_t* status) {
+                     cudaStream_t st, bool clear, int32_t* status, bool early) {
   const bool swiglu = w1 != nullptr;
   if (status == nullptr) status = static_cast<int32_t*>(scratch);
   if (int rc = check_int8_gemm(a, row_scale, offsets, w0, w1, scale0, scale1, M, K, N, E, dtype, out, status)) return rc;
@@ -696,7 +734,7 @@ int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offse
   if (int rc = small ? make_map_rows32(&ma, a, M, K) : make_map_a(&ma, a, M, K)) return rc;
   if (int rc = make_map_b(&mb0, w0, E, K, N)) return rc;
   if (int rc = make_map_b(&mb1, swiglu ? w1 : w0, E, K, N)) return rc;
-  const I8Params p{offsets, row_scale, scale0, scale1, out, status, E, M, K, N, n_tiles};
+  const I8Params p{offsets, row_scale, scale0, scale1, out, status, E, M, K, N, n_tiles, early && !clear};
   uint8_t* s = static_cast<uint8_t*>(scratch);
   const bool slabs = small || may_slice(M, n_tiles);
   const I8Slices sl{reinterpret_cast<uint32_t*>(s + kArrivalsAt), slabs ? reinterpret_cast<int4*>(s + kSlabsAt) : nullptr};

@@ -87,14 +87,21 @@ permute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ x, const int
 // R rows at a time and U pieces of each per thread: their places first, then their pieces, all requested before the first
 // is used.  Four to eight pieces in flight per thread, whatever K is (with R = 8 for two rows per token the registers that six absent
 // rows held kept half of the threads off the chip: 137 us for 16384 tokens x 2 rows of 4096, 61 us at the memory's rate).
+// Blocks of 128 threads, and rows that are read once marked as such where many are in flight (16384 x 2 rows: 75 us with the
+// mark, 70 without; 8192 x 8 rows of 2048: 50 and 58, 20000 x 4 rows of 1024: 30 and 35; 256 threads: 4 to 7 % more).
+constexpr int kSumThreads = 128;
+template <int R, class P> __device__ __forceinline__ P load_row(const P* p) {
+  if constexpr (R >= 4) return __ldcs(p);
+  else                  return *p;
+}
 template <class T, int BYTES, bool WEIGHTED, int R>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kSumThreads)
 unpermute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ rows, const int32_t* __restrict__ pos,
                       const float* __restrict__ weights, int n_tok, int K, int pieces, int lanes,
                       typename Piece<BYTES>::type* __restrict__ out) {
   constexpr int W = BYTES / (int)sizeof(T), U = kPiecesPerThread<R>;
   chain_wait();
-  const int t = blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes, c0 = blockIdx.y * lanes * U + threadIdx.x % lanes;
+  const int t = blockIdx.x * (kSumThreads / lanes) + threadIdx.x / lanes, c0 = blockIdx.y * lanes * U + threadIdx.x % lanes;
   if (t >= n_tok || c0 >= pieces) return;
   const int M = n_tok * K;
   float acc[U][W];
@@ -115,7 +122,7 @@ unpermute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ rows, cons
     for (int j = 0; j < R; ++j)
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (p[j] >= 0 && c0 + u * lanes < pieces) q[j][u].raw = rows[(size_t)p[j] * pieces + c0 + u * lanes];
+        if (p[j] >= 0 && c0 + u * lanes < pieces) q[j][u].raw = load_row<R>(rows + (size_t)p[j] * pieces + c0 + u * lanes);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       if (p[j] < 0) continue;
@@ -216,9 +223,9 @@ int piece_bytes(size_t row_bytes, std::initializer_list<const void*> ptrs) {
   for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
   return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
 }
-int lanes_for(int pieces) {
+int lanes_for(int pieces, int threads) {
   int lanes = 1;
-  while (lanes < pieces && lanes < kThreads) lanes *= 2;
+  while (lanes < pieces && lanes < threads) lanes *= 2;
   return lanes;
 }
 
@@ -241,7 +248,7 @@ template <int BYTES>
 int run_permute(const void* x, const int32_t* pos, const int32_t* offsets, int E, int T, int K, size_t row_bytes,
                 void* rows, cudaStream_t st) {
   using P = typename Piece<BYTES>::type;
-  const int pieces = (int)(row_bytes / BYTES), lanes = lanes_for(ceil_div(pieces, 2));
+  const int pieces = (int)(row_bytes / BYTES), lanes = lanes_for(ceil_div(pieces, 2), kThreads);
   const dim3 grid((unsigned)ceil_div(T, kThreads / lanes), (unsigned)ceil_div(pieces, 2 * lanes));
   BWMOE_REQUIRE(grid.y <= 65535, BWMOE_ERR_UNSUPPORTED, "permute_rows: rows of %zu bytes", row_bytes);
   BWMOE_CUDA_OK(launch_chained(permute_rows_kernel<BYTES>, grid, dim3(kThreads), 0, st, static_cast<const P*>(x), pos, offsets,
@@ -256,11 +263,11 @@ int run_unpermute(const void* rows, const int32_t* pos, const float* weights, in
   const int pieces = (int)(row_bytes / BYTES);
   auto run = [&](auto rows_at_once) {
     constexpr int R = decltype(rows_at_once)::value, U = kPiecesPerThread<R>;
-    const int lanes = lanes_for(ceil_div(pieces, U));
-    const dim3 grid((unsigned)ceil_div(n_tok, kThreads / lanes), (unsigned)ceil_div(pieces, U * lanes));
+    const int lanes = lanes_for(ceil_div(pieces, U), kSumThreads);
+    const dim3 grid((unsigned)ceil_div(n_tok, kSumThreads / lanes), (unsigned)ceil_div(pieces, U * lanes));
     BWMOE_REQUIRE(grid.y <= 65535, BWMOE_ERR_UNSUPPORTED, "unpermute_rows: rows of %zu bytes", row_bytes);
     auto kernel = weights ? unpermute_rows_kernel<T, BYTES, true, R> : unpermute_rows_kernel<T, BYTES, false, R>;
-    BWMOE_CUDA_OK(launch_chained(kernel, grid, dim3(kThreads), 0, st, static_cast<const P*>(rows), pos, weights, n_tok, K,
+    BWMOE_CUDA_OK(launch_chained(kernel, grid, dim3(kSumThreads), 0, st, static_cast<const P*>(rows), pos, weights, n_tok, K,
                                  pieces, lanes, static_cast<P*>(out)));
     return (int)BWMOE_OK;
   };

@@ -157,12 +157,14 @@ __device__ __forceinline__ uint4 piece_codes(const Piece16<T>& p, const RowScale
 }
 
 // wpr warps (1, 2, 4 or 8) share a row.  pos == nullptr: row t is written to row t.
+// next: the kernel behind is let in at once (a product that requests its weights meanwhile).
 template <class T>
 __global__ void __launch_bounds__(kThreads)
 quant_int8_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ pos, const int32_t* __restrict__ offsets, int E,
                        int n_tok, int K, int D, int wpr, int8_t* __restrict__ codes, float* __restrict__ scales,
-                       uint32_t* __restrict__ zero, int zero_words) {
+                       uint32_t* __restrict__ zero, int zero_words, bool next) {
   chain_wait();
+  if (next) chain_next();
   __shared__ uint32_t s_max[kThreads / 32];
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < zero_words; i += kThreads) zero[i] = 0u;
@@ -243,7 +245,7 @@ int launch_quant_int8_rows(const void* x, const int32_t* pos, const int32_t* off
   auto run = [&](auto tag) {
     using X = typename decltype(tag)::type;
     return launch_chained(quant_int8_rows_kernel<X>, grid, dim3(kThreads), 0, st, static_cast<const X*>(x), pos, offsets, E, T, K,
-                          D, wpr, static_cast<int8_t*>(codes), scales, static_cast<uint32_t*>(zero), (int)(zero_bytes / 4));
+                          D, wpr, static_cast<int8_t*>(codes), scales, static_cast<uint32_t*>(zero), (int)(zero_bytes / 4), (int)grid.x <= 2 * sm_count());
   };
   BWMOE_CUDA_OK(dtype == BWMOE_F32 ? run(TypeTag<float>{}) : dtype == BWMOE_F16 ? run(TypeTag<__half>{}) : run(TypeTag<__nv_bfloat16>{}));
   return BWMOE_OK;

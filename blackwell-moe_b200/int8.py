@@ -101,7 +101,7 @@ def int8_matmul(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor) -> tor
     code = _dtype_code(x, "x")
     dev = _require_cuda(_contig(x, "x"), _contig(w, "w"), _contig(w_scales, "w_scales"))
     (T, K), N = x.shape, w.shape[1]
-    out = torch.empty((T, N), dtype=x.dtype, device=dev)
+    out = x.new_empty((T, N))
     if T == 0:
         return out
     lib = _lib.lib()

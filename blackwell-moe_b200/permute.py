@@ -38,11 +38,11 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _empty_plan(T, K, num_experts, scratch_bytes, dev):
+def _empty_plan(indices, T, K, num_experts, scratch_bytes):
     """The plan's tensors, and the addresses of its status word and scratch behind them: one allocation."""
     M, extra = T * K, 4 + (scratch_bytes + 3) // 4
-    o, p, s, e, rest = torch.empty(num_experts + 1 + 3 * M + extra, dtype=torch.int32, device=dev).split(
-        (num_experts + 1, M, M, M, extra))
+    # (not views of one another: each has its own version, as tensors that were allocated apart)
+    o, p, s, e, rest = torch.unsafe_split_with_sizes(indices.new_empty(num_experts + 1 + 3 * M + extra), (num_experts + 1, M, M, M, extra))
     status = rest.data_ptr()
     return PermutePlan(o, p.view(T, K), s, e), status, status + 16
 
@@ -70,7 +70,7 @@ def permute_plan(indices: torch.Tensor, num_experts: int) -> PermutePlan:
     T, K = indices.shape
     lib = _lib.lib()
     with _on_device(dev):
-        plan, status, scratch = _empty_plan(T, K, num_experts, lib.bwmoe_plan_scratch_bytes(T, num_experts, K), dev)
+        plan, status, scratch = _empty_plan(indices, T, K, num_experts, lib.bwmoe_plan_scratch_bytes(T, num_experts, K))
         if T == 0:
             plan.offsets.zero_()
             return plan
@@ -86,8 +86,8 @@ def _permute_new(x, indices, num_experts):
     D, dev = x.shape[1], x.device
     lib = _lib.lib()
     with _on_device(dev):
-        plan, status, scratch = _empty_plan(T, K, num_experts, lib.bwmoe_plan_scratch_bytes(T, num_experts, K), dev)
-        rows = torch.empty((T * K, D), dtype=x.dtype, device=dev)
+        plan, status, scratch = _empty_plan(indices, T, K, num_experts, lib.bwmoe_plan_scratch_bytes(T, num_experts, K))
+        rows = x.new_empty((T * K, D))
         pos = plan.pos.data_ptr()
         _lib.check(lib.bwmoe_permute_tokens(x.data_ptr(), indices.data_ptr(), T, D, num_experts, K, _DTYPES[x.dtype],
                                             plan.offsets.data_ptr(), pos, pos + 4 * T * K, pos + 8 * T * K, rows.data_ptr(),
@@ -100,7 +100,7 @@ def _permute(x, offsets, pos):
     T, K = pos.shape
     D, dev = x.shape[1], x.device
     with _on_device(dev):
-        rows = torch.empty((T * K, D), dtype=x.dtype, device=dev)
+        rows = x.new_empty((T * K, D))
         if T and D:
             _lib.check(_lib.lib().bwmoe_permute_rows(x.data_ptr(), pos.data_ptr(), offsets.data_ptr(), T, D, offsets.numel() - 1,
                                                      K, _DTYPES[x.dtype], rows.data_ptr(), _stream(dev)))
@@ -112,7 +112,7 @@ def _unpermute(rows, pos, weights):
     T, K = pos.shape
     D, dev = rows.shape[1], rows.device
     with _on_device(dev):
-        out = torch.empty((T, D), dtype=rows.dtype, device=dev)
+        out = rows.new_empty((T, D))
         if T and D:
             _lib.check(_lib.lib().bwmoe_unpermute_rows(rows.data_ptr(), pos.data_ptr(),
                                                        None if weights is None else weights.data_ptr(), T, D, K,
@@ -124,8 +124,8 @@ def _unpermute_backward(dout, rows, offsets, pos, weights, rows_grad, weights_gr
     T, K = pos.shape
     D, dev = dout.shape[1], dout.device
     with _on_device(dev):
-        drows = torch.empty((T * K, D), dtype=dout.dtype, device=dev) if rows_grad else None
-        dweights = torch.empty((T, K), dtype=torch.float32, device=dev) if weights_grad else None
+        drows = dout.new_empty((T * K, D)) if rows_grad else None
+        dweights = torch.empty_like(weights) if weights_grad else None
         if T and D:
             if rows_grad or weights_grad:
                 _lib.check(_lib.lib().bwmoe_unpermute_rows_backward(
