@@ -376,14 +376,14 @@ int check_int8_args(const char* who, const void* x, const void* wg, const void* 
 
 int run_int8_pipeline(const void* x, const float* weights, const int32_t* indices, const void* wg, const void* wu,
                       const void* wd, const float* sg, const float* su, const float* sd, int T, int D, int H, int E, int K,
-                      int dtype, void* out, void* ws, const Int8Layout& L, cudaStream_t st) {
+                      int dtype, void* out, void* ws, const Int8Layout& L, cudaStream_t st, bool cleared) {
   const int M = T * K;
   int32_t* status = at<int32_t>(ws, L.status);
   int32_t *offsets = at<int32_t>(ws, L.offsets), *pos = at<int32_t>(ws, L.pos);
   float *sx = at<float>(ws, L.sx), *sh = at<float>(ws, L.sh);
   int rc;
   if ((rc = launch_plan(indices, nullptr, T, E, K, offsets, pos, at<int32_t>(ws, L.row_slot), at<int32_t>(ws, L.row_expert),
-                        nullptr, status, at<void>(ws, L.plan_scratch), st)))
+                        nullptr, status, at<void>(ws, L.plan_scratch), st, nullptr, false, ws, cleared ? 0 : L.zero_end)))
     return rc;
   if ((rc = launch_quant_int8_rows(x, pos, offsets, T, D, E, K, dtype, at<void>(ws, L.xq), sx, st))) return rc;
   if ((rc = launch_int8_gemm(at<void>(ws, L.xq), sx, offsets, wg, wu, sg, su, M, D, H, E, dtype, at<void>(ws, L.h),
@@ -886,6 +886,8 @@ int bwmoe_permute_tokens(const void* x, const int32_t* indices, int T, int D, in
                 "permute_tokens: D=%d K=%d type %d", D, K, dtype);
   BWMOE_REQUIRE((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows)) % dtype_bytes(dtype) == 0, BWMOE_ERR_BAD_ALIGN,
                 "permute_tokens: a pointer is not aligned to its type");
+  if (T > 0 && E > 0 && K > 0 && D <= (1 << 20) && plan_permute_applicable(T, E, K))
+    return launch_plan_permute(x, indices, T, E, K, (size_t)D * dtype_bytes(dtype), offsets, pos, row_slot, row_expert, status, rows, st);
   if (int rc = launch_plan(indices, nullptr, T, E, K, offsets, pos, row_slot, row_expert, nullptr, status, scratch, st)) return rc;
   return launch_permute_rows(x, pos, offsets, T, D, E, K, dtype, rows, st);
 }
@@ -970,8 +972,7 @@ int bwmoe_moe_forward_int_routed(const void* x, const float* weights, const int3
     return rc;
   BWMOE_REQUIRE(weights && indices, BWMOE_ERR_NULL, "moe_forward_int_routed: routing is null");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  BWMOE_CUDA_OK(cudaMemsetAsync(ws, 0, L.zero_end, st));
-  return run_int8_pipeline(x, weights, indices, wg, wu, wd, sg, su, sd, T, D, H, E, K, dtype, out, ws, L, st);
+  return run_int8_pipeline(x, weights, indices, wg, wu, wd, sg, su, sd, T, D, H, E, K, dtype, out, ws, L, st, false);
 }
 
 int bwmoe_moe_forward_int(const void* x, const void* w_gate, const void* wg, const void* wu, const void* wd, const float* sg,
@@ -987,7 +988,7 @@ int bwmoe_moe_forward_int(const void* x, const void* w_gate, const void* wg, con
   if (int rc = launch_router(x, w_gate, T, D, E, K, weights, indices, nullptr, st, at<void>(ws, L.router_scratch),
                              L.router_scratch_bytes, at<int32_t>(ws, L.status), 0, 0, ws, L.zero_end, at<void>(ws, L.router_head)))
     return rc;
-  return run_int8_pipeline(x, weights, indices, wg, wu, wd, sg, su, sd, T, D, H, E, K, BWMOE_BF16, out, ws, L, st);
+  return run_int8_pipeline(x, weights, indices, wg, wu, wd, sg, su, sd, T, D, H, E, K, BWMOE_BF16, out, ws, L, st, true);
 }
 
 }  // extern "C"

@@ -164,7 +164,8 @@ int launch_router_fallback(const void* x, const void* wg, const void* wgt, int D
 size_t plan_scratch_bytes(int T, int E, int K);
 int launch_plan(const int32_t* indices, const float* row_amax, int T, int E, int K, int32_t* offsets,
                 int32_t* pos, int32_t* row_slot, int32_t* row_expert, float* seg_amax, int32_t* status,
-                void* scratch, cudaStream_t st, float* scales_out = nullptr, bool amax_is_zero = false);
+                void* scratch, cudaStream_t st, float* scales_out = nullptr, bool amax_is_zero = false, void* zero = nullptr,
+                size_t zero_bytes = 0);      // zero: words cleared before the status can be raised
 // Plan and quantisation of a decode-sized batch in one launch (x_inv != nullptr: the block-scale recipe).  Only inside
 // the whole-block forwards: x is read before the kernel in front of it has finished.
 bool plan_quant_applicable(int T, int E, int K);
@@ -285,6 +286,10 @@ int launch_scatter_rows_group_peers(const void* xq_tok, const float* inv_tok, co
                                     int experts_per_rank, void* const* xq_of_rank, void* const* inv_of_rank,
                                     int n_ranks, int rows_cap, int32_t* status, cudaStream_t st);
 
+// Plan and copy of a decode-sized batch in one launch
+bool plan_permute_applicable(int T, int E, int K);
+int launch_plan_permute(const void* x, const int32_t* indices, int T, int E, int K, size_t row_bytes, int32_t* offsets, int32_t* pos,
+                        int32_t* row_slot, int32_t* row_expert, int32_t* status, void* rows, cudaStream_t st);
 // Tokens into expert order and back (permute_rows.cu)
 int launch_permute_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
                         void* rows, cudaStream_t st);

@@ -11,19 +11,12 @@
 // written as zeros.
 #include <type_traits>
 
-#include "common.cuh"
+#include "pieces.cuh"
 
 namespace bwmoe {
 namespace {
 
 constexpr int kThreads = 256;
-
-// A row is moved in pieces of 16 bytes; of 8, 4 or 2 where its length or a pointer allows no more.
-template <int BYTES> struct Piece;
-template <> struct Piece<16> { using type = uint4; };
-template <> struct Piece<8> { using type = uint2; };
-template <> struct Piece<4> { using type = uint32_t; };
-template <> struct Piece<2> { using type = uint16_t; };
 
 template <class T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -40,12 +33,6 @@ union Values {
   T v[BYTES / sizeof(T)];
   __device__ Values() {}
 };
-
-template <class P> __device__ __forceinline__ P zero_piece() {
-  P z;
-  memset(&z, 0, sizeof(P));
-  return z;
-}
 
 template <int ROWS> constexpr int kPiecesPerThread = ROWS >= 4 ? 8 / ROWS : 2;
 
@@ -217,12 +204,6 @@ unpermute_rows_backward_kernel(const typename Piece<BYTES>::type* __restrict__ d
   }
 }
 
-// Bytes of the widest piece that divides the row and every pointer.
-int piece_bytes(size_t row_bytes, std::initializer_list<const void*> ptrs) {
-  uintptr_t bits = (uintptr_t)row_bytes;
-  for (const void* p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
-  return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
-}
 int lanes_for(int pieces, int threads) {
   int lanes = 1;
   while (lanes < pieces && lanes < threads) lanes *= 2;
