@@ -101,6 +101,8 @@ def lib() -> C.CDLL:
     """Load the shared library once.  Raises if it has not been built: there is
     no other implementation to fall back to."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not _LIB_PATH.exists():

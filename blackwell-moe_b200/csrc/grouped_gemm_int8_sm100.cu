@@ -9,7 +9,7 @@
 //
 // Two kernels, persistent, one CTA per SM, warp-specialised (TMA producer, tcgen05.mma kind::i8 issuer, epilogue warps);
 // activations are read K-major, weights in the caller's [E, K, N] layout (N contiguous):
-//   int8_gemm_kernel        128 rows x 256 channels per tile, the rows on the MMA's M side
+//   int8_gemm_kernel        128 rows x 256 channels per tile, the rows on the MMA's M side; or a CTA pair on 256 x 256
 //   int8_gemm_small_kernel  32 rows x 256 channels per tile, the channels on the M side (decode batches)
 // (SWIGLU: 128 gate + 128 up channels in the place of the 256.)
 //
@@ -34,6 +34,7 @@ using namespace sm100;
 constexpr uint32_t IDESC_I8 = (2u << 4) | (1u << 7) | (1u << 10) | (0u << 15) | (1u << 16) | ((uint32_t)(BN >> 3) << 17) |
                               ((uint32_t)(BM >> 4) << 24);
 constexpr uint32_t IDESC_I8_HALF = (IDESC_I8 & ~(0x3fu << 17)) | ((uint32_t)(BN_HALF >> 3) << 17);      // N = 128: one weight box
+constexpr uint32_t IDESC_I8_PAIR = (IDESC_I8 & ~(0x1fu << 24)) | ((uint32_t)((2 * BM) >> 4) << 24);        // M = 256: a CTA pair
 constexpr int kMaxGroups = 256;
 constexpr int EPI_WARPS = 8;
 constexpr int I8_THREADS = 64 + 32 * EPI_WARPS;
@@ -43,6 +44,15 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -135,9 +145,9 @@ struct I8Pieces {
 
 // The weights of the CTA's first stages (all stages are free then); the number of stages begun.
 template <class Load>
-__device__ __forceinline__ int first_weights(I8Pieces q, int stages, Load load_weights) {
+__device__ __forceinline__ int first_weights(I8Pieces q, int stages, int first_piece, int piece_step, Load load_weights) {
   int n = 0;
-  for (long long piece = blockIdx.x; n < stages && piece < q.total; piece += gridDim.x) {
+  for (long long piece = first_piece; n < stages && piece < q.total; piece += piece_step) {
     q.locate(piece);
     for (int kb = q.kb0; n < stages && kb < q.kb1; ++kb, ++n) load_weights(q, kb, n);
   }
@@ -243,7 +253,12 @@ constexpr int L_MAX_PIECES = 320;                                             //
 constexpr int L_PART = BN / 2 * 32 / 4;                                       // vectors of one epilogue warp's part of a slab
 constexpr size_t L_SLAB = (size_t)EPI_WARPS * L_PART * sizeof(int4);          // 128 KiB
 
-template <bool SWIGLU, class T>
+// PAIR: the CTAs of a two-CTA cluster share 256-row tiles (cta_group::2).  CTA `rank` of the pair loads rows rank * 128 .. of the
+// tile and one of its two weight boxes (SWIGLU: rank 0 the gate's, rank 1 the up matrix's); the even CTA issues M = 256 MMAs
+// that read both shared memories and write each CTA's 128 rows into that CTA's tensor memory.  Loads of both CTAs report to
+// the even CTA's full barrier; the issuer commits to each CTA's empty and full-accumulator barriers in turn; the odd CTA's
+// epilogue warps hand accumulator buffers back on the even CTA's barrier.  None of the loads is a multicast.
+template <bool SWIGLU, class T, bool PAIR>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b0,
                  const __grid_constant__ CUtensorMap map_b1, const I8Params p, const I8Slices sl) {
@@ -254,38 +269,51 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort, s_per;
 
+  constexpr int NSTAGE = PAIR ? PAIR_STAGES : STAGES, STAGE_SZ = PAIR ? PAIR_STAGE_BYTES : STAGE_BYTES;
   const uint32_t tiles_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bars = tiles_base + STAGES * STAGE_BYTES;
-  const uint32_t bar_full = bars, bar_empty = bars + 8 * STAGES;
-  const uint32_t bar_tfull = bars + 16 * STAGES, bar_tempty = bar_tfull + 16;
+  const uint32_t bars = tiles_base + NSTAGE * STAGE_SZ;
+  const uint32_t bar_full = bars, bar_empty = bars + 8 * NSTAGE;
+  const uint32_t bar_tfull = bars + 16 * NSTAGE, bar_tempty = bar_tfull + 16;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;            // place in the pair
+  const int first_piece = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, piece_step = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k_blocks = (p.Kdim + BK - 1) / BK;
   volatile int* abort_flag = &s_abort;
 
   if (threadIdx.x == 0) {
     s_abort = 0;
-    for (int s = 0; s < STAGES; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 1);
-    for (int b = 0; b < 2; ++b) mbar_init(bar_tfull + 8 * b, 1), mbar_init(bar_tempty + 8 * b, EPI_WARPS);
+    for (int s = 0; s < NSTAGE; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 1);
+    for (int b = 0; b < 2; ++b) mbar_init(bar_tfull + 8 * b, 1), mbar_init(bar_tempty + 8 * b, PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  tile_table<I8_THREADS>(p, BM, p.n_tiles, s_first, s_end, s_cum);
+  tile_table<I8_THREADS>(p, PAIR ? 2 * BM : BM, p.n_tiles, s_first, s_end, s_cum);
   if (warp == 0) {
     __syncwarp();
-    const int per = sl.slabs == nullptr ? k_blocks : blocks_per_slice(s_cum[p.E], k_blocks, gridDim.x, L_MAX_PIECES, 3000, 2200);
+    const int per = PAIR || sl.slabs == nullptr ? k_blocks : blocks_per_slice(s_cum[p.E], k_blocks, gridDim.x, L_MAX_PIECES, 3000, 2200);
     if (lane == 0) s_per = per;
   }
-  if (warp == 1) tmem_alloc(smem_u32(&s_tmem_base), TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (PAIR) tmem_alloc_pair(smem_u32(&s_tmem_base), TMEM_COLS);
+    else                tmem_alloc(smem_u32(&s_tmem_base), TMEM_COLS);
+  }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();       // the peer's barriers and tensor memory exist from here on
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
-  I8Pieces q(s_first, s_end, s_cum, p.E, BM, k_blocks, s_per);
+  I8Pieces q(s_first, s_end, s_cum, p.E, PAIR ? 2 * BM : BM, k_blocks, s_per);
 
   // PLAIN: the last tile of a row may have one weight box of channels only; then the other is neither loaded nor multiplied
-  auto one_box = [&](const I8Pieces& q) { return !SWIGLU && q.n_idx * BN + BN_HALF >= p.N; };
+  auto one_box = [&](const I8Pieces& q) { return !SWIGLU && !PAIR && q.n_idx * BN + BN_HALF >= p.N; };
   auto load_weights = [&](const I8Pieces& q, int kb, uint32_t stage) {
-    const uint32_t sb = tiles_base + stage * STAGE_BYTES + A_BYTES, full = bar_full + 8 * stage;
+    const uint32_t sb = tiles_base + stage * STAGE_SZ + A_BYTES, full = bar_full + 8 * stage;
     const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN);
+    if constexpr (PAIR) {       // both CTAs' bytes are counted by the even CTA's barrier, which alone announces them
+      if (rank == 0) mbar_expect_tx(full, 2 * PAIR_STAGE_BYTES);
+      if (SWIGLU) tma_load_3d_pair(sb, rank ? &map_b1 : &map_b0, map_to_cta(full, 0), n0, kb * BK, q.e);
+      else        tma_load_3d_pair(sb, &map_b0, map_to_cta(full, 0), n0 + (int)rank * BN_HALF, kb * BK, q.e);
+      return;
+    }
     const bool one = one_box(q);
     mbar_expect_tx(full, one ? STAGE_BYTES - B_HALF_BYTES : STAGE_BYTES);
     tma_load_3d(sb, &map_b0, full, n0, kb * BK, q.e);
@@ -294,7 +322,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   };
   int ahead = 0;                // stages whose weights are on their way already
   if (p.early) {
-    if (threadIdx.x == 0) ahead = first_weights(q, STAGES, load_weights);
+    if (threadIdx.x == 0) ahead = first_weights(q, NSTAGE, first_piece, piece_step, load_weights);
     chain_wait();
   }
   if (warp == 0) {
@@ -302,7 +330,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     if (lane == 0) {
       uint32_t stage = 0, phase = 0;
       bool ok = true;
-      for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x) {
+      for (long long piece = first_piece; ok && piece < q.total; piece += piece_step) {
         q.locate(piece);
         for (int kb = q.kb0; kb < q.kb1; ++kb) {
           if (ahead > 0) {
@@ -311,17 +339,26 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status))) break;
             load_weights(q, kb, stage);
           }
-          tma_load_2d(tiles_base + stage * STAGE_BYTES, &map_a, bar_full + 8 * stage, kb * BK, q.row0);
-          if (++stage == STAGES) stage = 0, phase ^= 1u;
+          const uint32_t sa = tiles_base + stage * STAGE_SZ, full = bar_full + 8 * stage;
+          if constexpr (PAIR) tma_load_2d_pair(sa, &map_a, map_to_cta(full, 0), kb * BK, q.row0 + (int)rank * BM);
+          else                tma_load_2d(sa, &map_a, full, kb * BK, q.row0);
+          if (++stage == NSTAGE) stage = 0, phase ^= 1u;
+        }
+      }
+      if constexpr (PAIR) {
+        // the issuer's last commits arrive on this CTA's empty barriers from the other CTA: let them land before this CTA can leave
+        for (int i = 0; ok && i < NSTAGE; ++i) {
+          ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status);
+          if (++stage == NSTAGE) stage = 0, phase ^= 1u;
         }
       }
     }
   } else if (warp == 1) {
     // ===================== MMA issuer =====================
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       uint32_t stage = 0, phase = 0, local = 0;
       bool ok = true;
-      for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x, ++local) {
+      for (long long piece = first_piece; ok && piece < q.total; piece += piece_step, ++local) {
         q.locate(piece);
         const uint32_t buf = local & 1u, use = local >> 1, desc = one_box(q) ? IDESC_I8_HALF : IDESC_I8;
         if (!(ok = mbar_wait(bar_tempty + 8 * buf, (use & 1u) ^ 1u, abort_flag, p.status))) break;
@@ -329,15 +366,22 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         for (int kb = q.kb0; kb < q.kb1; ++kb) {
           if (!(ok = mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status))) break;
           tc_fence_after();
-          const uint32_t sa = tiles_base + stage * STAGE_BYTES;
+          const uint32_t sa = tiles_base + stage * STAGE_SZ;
           const uint64_t da = desc_kmajor(sa), db = desc_nmajor(sa + A_BYTES);
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)     // A: +32 bytes along K inside the swizzle atom; B: +32 K rows = 4096 bytes
-            mma_i8(tmem_base + buf * BN, da + (uint64_t)(k * 2), db + (uint64_t)(k * 256), desc, kb > q.kb0 || k > 0 ? 1u : 0u);
-          mma_commit(bar_empty + 8 * stage);
-          if (++stage == STAGES) stage = 0, phase ^= 1u;
+          for (int k = 0; k < BK / 32; ++k) {   // A: +32 bytes along K inside the swizzle atom; B: +32 K rows = 4096 bytes
+            const uint32_t acc = kb > q.kb0 || k > 0 ? 1u : 0u;
+            if constexpr (PAIR) mma_i8_pair(tmem_base + buf * BN, da + (uint64_t)(k * 2), db + (uint64_t)(k * 256), IDESC_I8_PAIR, acc);
+            else                mma_i8(tmem_base + buf * BN, da + (uint64_t)(k * 2), db + (uint64_t)(k * 256), desc, acc);
+          }
+          if constexpr (PAIR) mma_commit_pair(bar_empty + 8 * stage), mma_commit_pair(map_to_cta(bar_empty + 8 * stage, 1));
+          else                mma_commit(bar_empty + 8 * stage);
+          if (++stage == NSTAGE) stage = 0, phase ^= 1u;
         }
-        if (ok) mma_commit(bar_tfull + 8 * buf);
+        if (ok) {
+          if constexpr (PAIR) mma_commit_pair(bar_tfull + 8 * buf), mma_commit_pair(map_to_cta(bar_tfull + 8 * buf, 1));
+          else                mma_commit(bar_tfull + 8 * buf);
+        }
       }
     }
   } else {
@@ -346,10 +390,10 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     float* my_scale = s_scale[warp - 2];
     uint32_t local = 0;
     bool ok = true;
-    for (long long piece = blockIdx.x; ok && piece < q.total; piece += gridDim.x, ++local) {
+    for (long long piece = first_piece; ok && piece < q.total; piece += piece_step, ++local) {
       q.locate(piece);
       const uint32_t buf = local & 1u, use = local >> 1;
-      const int row = q.row0 + quarter * 32 + lane;
+      const int row = q.row0 + (int)rank * BM + quarter * 32 + lane;
       const bool row_ok = row < q.row_end;
       const float rs = row_ok ? p.row_scale[row] : 0.f;
       // channel scales of this warp's columns (SWIGLU: 64 of the gate, then 64 of the up product), zero past N
@@ -429,7 +473,10 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
+      if (lane == 0) {
+        if (PAIR && rank != 0) mbar_arrive_cluster(map_to_cta(bar_tempty + 8 * buf, 0));
+        else                   mbar_arrive(bar_tempty + 8 * buf);
+      }
     }
     zero_tail_rows<T>(p, blockIdx.x * (32 * EPI_WARPS) + threadIdx.x - 64, gridDim.x * (32 * EPI_WARPS));
   }
@@ -440,8 +487,12 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();       // neither CTA leaves while the other may still signal it
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else                tmem_dealloc(tmem_base, TMEM_COLS);
+  }
 }
 
 // ---------------------------------------------------------------- few rows per expert
@@ -513,7 +564,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
   };
   int ahead = 0;                // stages whose weights are on their way already
   if (p.early) {
-    if (threadIdx.x == 0) ahead = first_weights(q, S_STAGES, load_weights);
+    if (threadIdx.x == 0) ahead = first_weights(q, S_STAGES, blockIdx.x, gridDim.x, load_weights);
     chain_wait();
   }
   if (warp == 0) {
@@ -666,22 +717,78 @@ bool may_slice(int M, int n_tiles) { return (long long)ceil_div(M, BM) * n_tiles
 constexpr size_t kArrivalsAt = 16;
 constexpr size_t kSlabsAt = kArrivalsAt + (S_MAX_PIECES > L_MAX_PIECES ? S_MAX_PIECES : L_MAX_PIECES) / 2 * EPI_WARPS * sizeof(uint32_t);
 
+// CTA pairs (256-row tiles, every weight byte enters one of the two shared memories) take a third of the traffic into the SMs
+// away: an SM takes in about 64 bytes a cycle, and a 128 x 256 tile alone asks for 96 while its MMAs run.  They pay in products
+// long enough to run at the power limit; in short ones what they add at either end of a tile costs more, and with few rows
+// per expert the rows past a segment's end do.  Measured, us, pairs against single CTAs (alternating, queued back to back):
+//   8 experts, 4096 rows each:  4096 x 14336 SwiGLU 2740 / 3000,  14336 x 4096 1560 / 1660;  2048 rows each: 1390 / 1490, 705 / 760
+//   one matrix, 8192 rows:  8192 x 8192 368 / 454,  4096 x 14336 334 / 380,  1024 x 8192 100 / 82;  4096 rows, 8192 x 8192: 216 / 199
+//   64 experts, 768 rows each, 2048 x 1408 SwiGLU 328 / 301;  1024 rows each of 8 x 4096 x 14336 SwiGLU 852 / 775
+constexpr int kPairMinRows = 2048;                     // per expert
+constexpr double kPairMinProducts = 4e11;
+bool pair_applies(int M, int K, int N, int E, bool swiglu) {
+  return (long long)M >= (long long)kPairMinRows * E && (double)M * K * N * (swiglu ? 2 : 1) >= kPairMinProducts &&
+         (swiglu || N % BN == 0) && gemm_sm_budget() >= 2;
+}
+
 template <class Kernel>
-int run(Kernel kernel, bool small, const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1, const I8Params& p,
-        const I8Slices& sl, unsigned char (&smem_set)[64], cudaStream_t st) {
-  const int smem = small ? S_SMEM_BYTES : SMEM_BYTES, k_blocks = ceil_div(p.Kdim, BK);
+int run(Kernel kernel, dim3 grid, int threads, int smem, unsigned char (&smem_set)[64], const CUtensorMap& ma, const CUtensorMap& mb0,
+        const CUtensorMap& mb1, const I8Params& p, const I8Slices& sl, cudaStream_t st) {
   BWMOE_CUDA_OK(ensure_dynamic_smem(kernel, smem, smem_set));
-  const long long max_pieces = (long long)(ceil_div(p.M, small ? S_NT : BM) + p.E) * p.n_tiles * (sl.slabs ? k_blocks : 1);
-  const int grid = (int)std::min<long long>(gemm_sm_budget(), max_pieces);
-  BWMOE_CUDA_OK(launch_chained(kernel, dim3(grid), dim3(small ? S_THREADS : I8_THREADS), smem, st, ma, mb0, mb1, p, sl));
+  BWMOE_CUDA_OK(launch_chained(kernel, grid, dim3(threads), smem, st, ma, mb0, mb1, p, sl));
   return BWMOE_OK;
 }
+
+template <class Kernel>
+int run_pair(Kernel kernel, unsigned char (&smem_set)[64], int (&resident)[64], const CUtensorMap& ma, const CUtensorMap& mb0,
+             const CUtensorMap& mb1, const I8Params& p, const I8Slices& sl, cudaStream_t st) {
+  BWMOE_CUDA_OK(ensure_dynamic_smem(kernel, PAIR_SMEM_BYTES, smem_set));
+  const long long max_tiles = (long long)(ceil_div(p.M, 2 * BM) + p.E) * p.n_tiles;
+  int pairs = (int)std::min<long long>(gemm_sm_budget() / 2, max_tiles);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(I8_THREADS);
+  cfg.dynamicSmemBytes = PAIR_SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;     // the kernel waits for the one in front
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  // pairs that can be resident at once (per device, asked once): the persistent loop needs no more
+  int dev = 0;
+  BWMOE_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64) {
+    if (resident[dev] == 0) {
+      int n = 0;
+      cfg.gridDim = dim3(2 * (sm_count() / 2));
+      BWMOE_CUDA_OK(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+      BWMOE_REQUIRE(n >= 1, BWMOE_ERR_CUDA, "no CTA pair of the 8-bit integer product fits on this device");
+      resident[dev] = n;
+    }
+    pairs = std::min(pairs, resident[dev]);
+  }
+  cfg.gridDim = dim3(2 * pairs);
+  note_launch();
+  BWMOE_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, ma, mb0, mb1, p, sl));
+  return BWMOE_OK;
+}
+
 template <bool SWIGLU, class T>
 int run_typed(bool small, const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1, const I8Params& p,
               const I8Slices& sl, cudaStream_t st) {
-  static unsigned char smem_set[2][64] = {};
-  return small ? run(int8_gemm_small_kernel<SWIGLU, T>, true, ma, mb0, mb1, p, sl, smem_set[1], st)
-               : run(int8_gemm_kernel<SWIGLU, T>, false, ma, mb0, mb1, p, sl, smem_set[0], st);
+  static unsigned char smem_set[3][64] = {};
+  static int resident[64] = {};
+  if (!small && pair_applies(p.M, p.Kdim, p.N, p.E, SWIGLU))
+    return run_pair(int8_gemm_kernel<SWIGLU, T, true>, smem_set[2], resident, ma, mb0, mb1, p, sl, st);
+  const long long max_pieces = (long long)(ceil_div(p.M, small ? S_NT : BM) + p.E) * p.n_tiles * (sl.slabs ? ceil_div(p.Kdim, BK) : 1);
+  const dim3 grid((unsigned)std::min<long long>(gemm_sm_budget(), max_pieces));
+  return small ? run(int8_gemm_small_kernel<SWIGLU, T>, grid, S_THREADS, S_SMEM_BYTES, smem_set[1], ma, mb0, mb1, p, sl, st)
+               : run(int8_gemm_kernel<SWIGLU, T, false>, grid, I8_THREADS, SMEM_BYTES, smem_set[0], ma, mb0, mb1, p, sl, st);
 }
 
 // fn(type tag)

@@ -16,8 +16,9 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxE = 256;
 constexpr int kPlanMaxBlocks = 256;
-// Slots ranked by one block, in rounds of 1024: one round while that keeps the blocks at 128 or fewer (a second one costs
-// 10.3 us instead of 6.9 for 8024 slots of 128 experts, 13.1 instead of 9.8 for 131072 of 256), two up to 256 blocks, more beyond, because every block adds up all blocks' histograms.
+// Slots ranked by one block, in rounds of 1024: one round while that keeps the blocks at 128 or fewer (with two rounds 8024
+// slots of 128 experts take 10.3 us instead of 6.9, 131072 of 256 experts 13.1 instead of 9.8), two up to 256 blocks, more
+// beyond, because every block adds up all blocks' histograms.
 constexpr int kPlanOneRoundBlocks = 128;
 inline int plan_slots_per_block(long long M) {
   if (M <= (long long)kPlanOneRoundBlocks * kPlanThreads) return kPlanThreads;

@@ -307,3 +307,48 @@ def test_segments_from_elsewhere_stay_inside_the_rows():
         if offsets[1:3] == [10, 30]:
             for e, (lo, hi) in enumerate(((0, 10), (10, 30), (30, 40))):
                 assert torch.equal(out[lo:hi].double(), a[lo:hi].double() @ w[e].double())
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("counts,loose,K,N", [([5000, 4000], 7, 4096, 8192), ([8200], 0, 8192, 6144), ([0, 3001, 257, 9000, 1], 300, 4096, 7680)])
+def test_long_products(counts, loose, K, N, swiglu):
+    """Products long enough for CTA pairs, with segments that end anywhere in a pair's tile; some rows are compared."""
+    M, E = sum(counts) + loose, len(counts)
+    offsets, _ = make_segments(counts, M)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    codes = lambda *shape: torch.randint(-128, 128, shape, generator=g, device=DEV, dtype=torch.int16).to(I8)     # noqa: E731
+    a, w, w2 = codes(M, K), codes(E, K, N), codes(E, K, N)
+    rs = torch.rand(M, generator=g, device=DEV) * 1e-2
+    cs, cs2 = (torch.rand(E, N, generator=g, device=DEV) * 2e-4 for _ in range(2))
+    if swiglu:
+        out = bw.int8_grouped_swiglu(a, rs, offsets.to(DEV), w, w2, cs, cs2)
+    else:
+        out = bw.int8_grouped_gemm(a, rs, offsets.to(DEV), w, cs)
+    for e in range(E):
+        lo, hi = int(offsets[e]), int(offsets[e + 1])
+        rows = sorted({r for r in (lo, lo + 1, lo + 127, lo + 128, lo + 255, lo + 256, (lo + hi) // 2, hi - 129, hi - 2, hi - 1) if lo <= r < hi})
+        if not rows:
+            continue
+        x, r = a[rows].double(), rs[rows, None].double()
+        gate = (x @ w[e].double()) * r * cs[e].double()
+        if swiglu:
+            ref, bound = swiglu_bound(gate, (x @ w2[e].double()) * r * cs2[e].double(), BF16)
+        else:
+            ref, bound = gate, gate.abs() * (3.01 * U32 + half_step(BF16) * 1.001) + smallest_step(BF16)
+        assert ((out[rows].double() - ref).abs() <= bound).all(), e
+    assert (out[sum(counts):] == 0).all()
+
+
+def test_quotients_of_all_pairs_of_16_bit_numbers():
+    """Rows whose largest value runs through every significand, with every smaller value from a 512th of it on: all the ties,
+    and all that lies next to one."""
+    for dtype, bits in ((BF16, 8), (F16, 11)):
+        ints = torch.arange(2 ** (bits - 1), 2 ** bits).float()
+        values = torch.cat([ints * 2.0 ** -s for s in range(1, 10)] + [ints])
+        x = values.repeat(len(ints), 1)
+        x[x > ints[:, None]] = 0
+        x[:, 1::2] *= -1
+        x[torch.arange(len(ints)), len(values) - len(ints) + torch.arange(len(ints))] = ints
+        for scale in (1.0, 2.0 ** -9):
+            y = (x * scale).to(dtype)
+            assert_codes(*bw.quantize_tokens_int8(y.to(DEV)), y)
