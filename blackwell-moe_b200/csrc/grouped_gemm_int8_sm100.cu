@@ -499,6 +499,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 // Few rows per expert (decode): bound by the weights' bytes.  The weight tile takes the M side of the MMA and the rows the N
 // side, D^T[128 channels (tensor-memory lanes), 32 rows (columns)]: a stage is 32 KiB of weights and 4 KiB of rows, and six of
 // them are in flight.  Two epilogue warps per lane quarter, 16 of the rows each; a thread owns a channel of either weight tile.
+// NARROW: 128 channels per tile, one weight box per stage, where that still fits the SMs at once: twice the tiles, half the
+// slices to add up (one row, 4096 x 14336: 17.5 -> 15.5 us, 2048 x 2048: 9.5 -> 8.6; 32 rows, 8192 x 1024: 16.5 -> 12.4).
 constexpr int S_NT = 32;                                     // rows per tile
 constexpr int S_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int S_STAGES = 6;
@@ -517,11 +519,13 @@ constexpr uint32_t IDESC_I8_SMALL = (2u << 4) | (1u << 7) | (1u << 10) | (1u << 
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[8]) { tmem_ld8(taddr, r); }
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
 
-template <bool SWIGLU, class T>
+template <bool SWIGLU, class T, bool NARROW>
 __global__ void __launch_bounds__(S_THREADS, 1)
 int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w0,
                        const __grid_constant__ CUtensorMap map_w1, const I8Params p, const I8Slices sl) {
   if (!p.early) chain_wait();
+  static_assert(!(SWIGLU && NARROW), "SwiGLU has two weight boxes");
+  constexpr int CH = SWIGLU || NARROW ? BN_HALF : BN;             // channels of the result in a tile
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_first[kMaxGroups], s_end[kMaxGroups], s_cum[kMaxGroups + 1];
   __shared__ uint32_t s_tmem_base;
@@ -556,11 +560,11 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
 
   auto load_weights = [&](const I8Pieces& q, int kb, uint32_t stage) {
     const uint32_t sw = tiles_base + stage * S_STAGE_BYTES, full = bar_full + 8 * stage;
-    const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN);
-    mbar_expect_tx(full, S_STAGE_BYTES);
+    const int n0 = q.n_idx * CH;
+    mbar_expect_tx(full, NARROW ? S_STAGE_BYTES - B_HALF_BYTES : S_STAGE_BYTES);
     tma_load_3d(sw, &map_w0, full, n0, kb * BK, q.e);
-    if (SWIGLU) tma_load_3d(sw + B_HALF_BYTES, &map_w1, full, n0, kb * BK, q.e);
-    else        tma_load_3d(sw + B_HALF_BYTES, &map_w0, full, n0 + BN_HALF, kb * BK, q.e);
+    if (SWIGLU)       tma_load_3d(sw + B_HALF_BYTES, &map_w1, full, n0, kb * BK, q.e);
+    else if (!NARROW) tma_load_3d(sw + B_HALF_BYTES, &map_w0, full, n0 + BN_HALF, kb * BK, q.e);
   };
   int ahead = 0;                // stages whose weights are on their way already
   if (p.early) {
@@ -605,7 +609,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k) {     // weights: +32 K rows = 4096 bytes; rows: +32 bytes along K
             mma_i8(d, da0 + (uint64_t)(k * 256), db + (uint64_t)(k * 2), IDESC_I8_SMALL, kb > q.kb0 || k > 0 ? 1u : 0u);
-            mma_i8(d + S_NT, da1 + (uint64_t)(k * 256), db + (uint64_t)(k * 2), IDESC_I8_SMALL, kb > q.kb0 || k > 0 ? 1u : 0u);
+            if (!NARROW) mma_i8(d + S_NT, da1 + (uint64_t)(k * 256), db + (uint64_t)(k * 2), IDESC_I8_SMALL, kb > q.kb0 || k > 0 ? 1u : 0u);
           }
           mma_commit(bar_empty + 8 * stage);
           if (++stage == S_STAGES) stage = 0, phase ^= 1u;
@@ -622,9 +626,9 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       q.locate(piece);
       const uint32_t buf = it % S_NBUF, use = it / S_NBUF;
       const int n_valid = min(S_NT / 2, q.row_end - q.row0 - c0);       // this warp's rows; none: <= 0
-      const int n = q.n_idx * (SWIGLU ? BN_HALF : BN) + f, m = SWIGLU ? n : n + BN_HALF;      // the thread's two channels
+      const int n = q.n_idx * CH + f, m = SWIGLU ? n : n + BN_HALF;      // the thread's two channels (NARROW: the first)
       const float s0 = n < p.N ? p.scale0[(size_t)q.e * p.N + n] : 0.f;
-      const float s1 = m < p.N ? (SWIGLU ? p.scale1 : p.scale0)[(size_t)q.e * p.N + m] : 0.f;
+      const float s1 = !NARROW && m < p.N ? (SWIGLU ? p.scale1 : p.scale0)[(size_t)q.e * p.N + m] : 0.f;
       const float my_rs = lane < n_valid ? p.row_scale[q.row0 + c0 + lane] : 0.f;
       ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * buf, use & 1u, abort_flag, p.status));
       if (!ok) break;
@@ -634,7 +638,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         constexpr int NC = decltype(columns)::value;
         uint32_t a0[NC], a1[NC];
         tmem_ld_cols(t_row, a0);
-        tmem_ld_cols(t_row + S_NT, a1);
+        if (!NARROW) tmem_ld_cols(t_row + S_NT, a1);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
@@ -643,22 +647,22 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
           const int4* part0 = sl.slabs + ((size_t)q.tile * q.slices * EPI_WARPS + (warp - 2)) * S_PART;
           int4* part = const_cast<int4*>(part0) + (size_t)q.slice * EPI_WARPS * S_PART;
           slab_store<NC>(part, 0, lane, a0);
-          slab_store<NC>(part, S_NT / 8, lane, a1);
+          if (!NARROW) slab_store<NC>(part, S_NT / 8, lane, a1);
           if (!last_slice(sl.arrivals + q.tile * EPI_WARPS + (warp - 2), q.slices, lane)) return;
           slab_add<NC>(part0, (size_t)EPI_WARPS * S_PART, q.slices, q.slice, 0, lane, a0);
-          slab_add<NC>(part0, (size_t)EPI_WARPS * S_PART, q.slices, q.slice, S_NT / 8, lane, a1);
+          if (!NARROW) slab_add<NC>(part0, (size_t)EPI_WARPS * S_PART, q.slices, q.slice, S_NT / 8, lane, a1);
         }
         T* out = static_cast<T*>(p.out) + (size_t)(q.row0 + c0) * p.N;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const float rs = __shfl_sync(0xffffffffu, my_rs, c);
-          const float v0 = __int2float_rn((int)a0[c]) * rs * s0, v1 = __int2float_rn((int)a1[c]) * rs * s1;
+          const float v0 = __int2float_rn((int)a0[c]) * rs * s0, v1 = NARROW ? 0.f : __int2float_rn((int)a1[c]) * rs * s1;
           if (c >= n_valid) continue;
           if (SWIGLU) {
             if (n < p.N) out[(size_t)c * p.N + n] = Out<T>::one(swiglu<T>(v0, v1));
           } else {
             if (n < p.N) out[(size_t)c * p.N + n] = Out<T>::one(v0);
-            if (m < p.N) out[(size_t)c * p.N + m] = Out<T>::one(v1);
+            if (!NARROW && m < p.N) out[(size_t)c * p.N + m] = Out<T>::one(v1);
           }
         }
       };
@@ -709,6 +713,11 @@ bool small_applies(int M, int K, int n_tiles, int E) {
   if (M <= 32ll * E) return true;
   const long long tiles = ((long long)M / S_NT + E) * n_tiles;
   return tiles <= sm_count() && tiles * ceil_div(K, BK) <= 8192;
+}
+// 128 channels per tile: one product of one matrix (whose tiles are known here) and one or two row blocks (with three of K =
+// 14336 the rows' boxes count: 33 us against 28).
+bool narrow_applies(int M, int N, int E, bool swiglu) {
+  return !swiglu && E == 1 && M <= 2 * S_NT && ceil_div(M, S_NT) * ceil_div(N, BN_HALF) <= sm_count();
 }
 // Whether the other kernel's tiles may leave SMs without work, so that slabs are worth their memory.
 bool may_slice(int M, int n_tiles) { return (long long)ceil_div(M, BM) * n_tiles < sm_count(); }
@@ -787,7 +796,12 @@ int run_typed(bool small, const CUtensorMap& ma, const CUtensorMap& mb0, const C
     return run_pair(int8_gemm_kernel<SWIGLU, T, true>, smem_set[2], resident, ma, mb0, mb1, p, sl, st);
   const long long max_pieces = (long long)(ceil_div(p.M, small ? S_NT : BM) + p.E) * p.n_tiles * (sl.slabs ? ceil_div(p.Kdim, BK) : 1);
   const dim3 grid((unsigned)std::min<long long>(gemm_sm_budget(), max_pieces));
-  return small ? run(int8_gemm_small_kernel<SWIGLU, T>, grid, S_THREADS, S_SMEM_BYTES, smem_set[1], ma, mb0, mb1, p, sl, st)
+  if constexpr (!SWIGLU) {
+    static unsigned char narrow_set[64] = {};
+    if (small && p.n_tiles == ceil_div(p.N, BN_HALF) && p.n_tiles != ceil_div(p.N, BN))
+      return run(int8_gemm_small_kernel<false, T, true>, grid, S_THREADS, S_SMEM_BYTES, narrow_set, ma, mb0, mb1, p, sl, st);
+  }
+  return small ? run(int8_gemm_small_kernel<SWIGLU, T, false>, grid, S_THREADS, S_SMEM_BYTES, smem_set[1], ma, mb0, mb1, p, sl, st)
                : run(int8_gemm_kernel<SWIGLU, T, false>, grid, I8_THREADS, SMEM_BYTES, smem_set[0], ma, mb0, mb1, p, sl, st);
 }
 
@@ -841,7 +855,8 @@ int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offse
   if (int rc = small ? make_map_rows32(&ma, a, M, K) : make_map_a(&ma, a, M, K)) return rc;
   if (int rc = make_map_b(&mb0, w0, E, K, N)) return rc;
   if (int rc = make_map_b(&mb1, swiglu ? w1 : w0, E, K, N)) return rc;
-  const I8Params p{offsets, row_scale, scale0, scale1, out, status, E, M, K, N, n_tiles, early && !clear};
+  I8Params p{offsets, row_scale, scale0, scale1, out, status, E, M, K, N, n_tiles, early && !clear};
+  if (small && narrow_applies(M, N, E, swiglu)) p.n_tiles = ceil_div(N, BN_HALF);
   uint8_t* s = static_cast<uint8_t*>(scratch);
   const bool slabs = small || may_slice(M, n_tiles);
   const I8Slices sl{reinterpret_cast<uint32_t*>(s + kArrivalsAt), slabs ? reinterpret_cast<int4*>(s + kSlabsAt) : nullptr};
