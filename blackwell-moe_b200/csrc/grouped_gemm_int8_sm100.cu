@@ -84,7 +84,8 @@ __device__ __forceinline__ void tile_table(const I8Params& p, int tile_rows, int
     int r0 = 0, r1 = 0;
     if (e < p.E) segment(p, e, r0, r1);
     s_first[e] = r0, s_end[e] = r1;
-    s_cum[e + 1] = ((r1 - r0 + tile_rows - 1) / tile_rows) * tiles_per_row_block;
+    // (no result that fits the memory has 2^22 tiles; segments that overlap might, and the sum over them fits 32 bits so)
+    s_cum[e + 1] = (int)min((long long)((r1 - r0 + tile_rows - 1) / tile_rows) * tiles_per_row_block, 1ll << 22);
   }
   __syncthreads();
   if (threadIdx.x < 32) {       // inclusive scan: 8 values per lane, then a shuffle scan of the lanes' totals

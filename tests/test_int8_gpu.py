@@ -296,6 +296,58 @@ def test_streams_and_captured_graphs(T):
         assert all(torch.equal(a, b) for a, b in zip(captured, step()))
 
 
+@pytest.mark.parametrize("T", [3, 40, 600])
+def test_graphs_that_are_replayed_side_by_side(T):
+    """Two graphs captured on one stream, replayed on two at once: they have no workspace in common."""
+    D, H, E, K = 512, 1024, 8, 2
+    sets = [make_block(T, D, H, E, K, BF16, seed) for seed in (1, 2)]
+    graphs, outs = [], []
+    for x, weights, idx, ws, ss in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append((bw.int8_moe_forward_routed(x, weights, idx, *ws, *ss), bw.int8_matmul(x, ws[0][0], ss[0][0])))
+    want = [(bw.int8_moe_forward_routed(x, weights, idx, *ws, *ss), bw.int8_matmul(x, ws[0][0], ss[0][0]))
+            for x, weights, idx, ws, ss in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for got, ref in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_two_streams_at_once():
+    x, weights, idx, ws, ss = make_block(50, 512, 1024, 8, 2, BF16, 4)
+    want = bw.int8_moe_forward_routed(x, weights, idx, *ws, *ss)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(bw.int8_moe_forward_routed(x, weights, idx, *ws, *ss))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_the_same_workspace_for_batches_of_all_sizes():
+    """The stream's workspace carries what the call before left in it: sizes up and down, cut tiles and uncut ones."""
+    D, H, E, K = 512, 2048, 8, 2
+    x, weights, idx, ws, ss = make_block(1500, D, H, E, K, BF16, 6)
+    first = {}
+    for T in (1, 1500, 7, 130, 1, 513, 40, 1500, 130, 7, 513, 40):
+        out = bw.int8_moe_forward_routed(x[:T].contiguous(), weights[:T].contiguous(), idx[:T].contiguous(), *ws, *ss)
+        lin = bw.int8_matmul(x[:T].contiguous(), ws[0][3], ss[0][3])
+        if T in first:
+            assert torch.equal(out, first[T][0]) and torch.equal(lin, first[T][1])
+        first[T] = (out, lin)
+    # a token's row does not depend on the rows beside it, nor on the kernel that its batch got
+    assert torch.equal(first[1][1], first[1500][1][:1]) and torch.equal(first[130][0], first[1500][0][:130])
+
+
 def test_segments_from_elsewhere_stay_inside_the_rows():
     """Offsets past the rows, negative or falling: clamped, nothing is read or written out of range."""
     M, K, N, E = 40, 64, 64, 3

@@ -214,6 +214,68 @@ def test_another_stream_and_a_captured_graph():
         assert all(torch.equal(a, b) for a, b in zip(captured, step()))
 
 
+def test_a_captured_training_step():
+    """Forward and backward through autograd inside a graph, replayed on new values."""
+    T, D, E, K = 200, 128, 16, 2
+    idx, w = routing(T, E, K, 9)
+    idx = idx.to(DEV)
+    x, wt = torch.randn(T, D, device=DEV).to(BF16).requires_grad_(), w.to(DEV).requires_grad_()
+    grad = torch.randn(T, D, device=DEV).to(BF16)
+
+    def step():
+        rows, plan = bw.permute_tokens(x, idx, E)
+        out = bw.unpermute_tokens(rows * 2, plan, wt)
+        return (out.detach(), *torch.autograd.grad(out, (x, wt), grad))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(3):
+        new, w2 = routing(T, E, K, 40 + seed)
+        with torch.no_grad():
+            idx.copy_(new), wt.copy_(w2), x.normal_(), grad.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+
+
+def test_no_second_derivative():
+    idx, w = routing(6, 4, 2, 0)
+    x, wt = torch.randn(6, 40, device=DEV, requires_grad=True), w.to(DEV).requires_grad_()
+    rows, plan = bw.permute_tokens(x, idx.to(DEV), 4)
+    dx, = torch.autograd.grad(rows.square().sum(), x, create_graph=True)
+    assert torch.equal(dx.detach(), 4 * x.detach())
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), x)
+    out = bw.unpermute_tokens(rows.detach(), plan, wt)
+    dw, = torch.autograd.grad(out.square().sum(), wt, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dw.sum(), wt)
+
+
+def test_a_value_changed_before_the_backward_pass_is_noticed():
+    idx, w = routing(6, 4, 2, 0)
+    r, wt = torch.randn(12, 40, device=DEV, requires_grad=True), w.to(DEV).requires_grad_()
+    plan = bw.permute_plan(idx.to(DEV), 4)
+    out = bw.unpermute_tokens(r, plan, wt)
+    with torch.no_grad():
+        wt.mul_(2)
+    with pytest.raises(RuntimeError):
+        out.sum().backward()
+    rows, plan = bw.permute_tokens(r, torch.zeros(12, 1, dtype=torch.int32, device=DEV), 2)
+    plan.offsets.zero_()                          # not needed by the backward pass: each tensor of a plan stands for itself
+    rows.sum().backward()
+    rows, plan = bw.permute_tokens(r, torch.zeros(12, 1, dtype=torch.int32, device=DEV), 2)
+    plan.pos.zero_()
+    with pytest.raises(RuntimeError):
+        rows.sum().backward()
+
+
 def test_rows_beyond_two_to_the_thirty_one_values():
     T, D, E, K = 34000, 8192, 8, 8
     idx, w = routing(T, E, K, 6)
