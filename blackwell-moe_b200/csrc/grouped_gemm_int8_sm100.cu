@@ -240,14 +240,15 @@ template <class T> __device__ __forceinline__ float swiglu(float g, float u) {
   else                          return silu_f(g) * u;
 }
 
-// Rows behind the last segment belong to no expert: zeros.  `part` of `parts` threads.
+// Rows in front of the first segment and behind the last belong to no expert: zeros.  `part` of `parts` threads.
 template <class T>
-__device__ __forceinline__ void zero_tail_rows(const I8Params& p, int part, int parts) {
+__device__ __forceinline__ void zero_other_rows(const I8Params& p, int part, int parts) {
   if (p.offsets == nullptr) return;
-  const int first = min(max(p.offsets[p.E], 0), p.M);
-  const size_t n = (size_t)(p.M - first) * p.N / Out<T>::kPer16;
-  uint4* at = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (size_t)first * p.N);
-  for (size_t i = part; i < n; i += parts) at[i] = make_uint4(0u, 0u, 0u, 0u);
+  const size_t row = (size_t)p.N / Out<T>::kPer16;      // 16-byte vectors
+  const size_t head = min(max(p.offsets[0], 0), p.M) * row, tail = min(max(p.offsets[p.E], 0), p.M) * row, end = p.M * row;
+  uint4* out = static_cast<uint4*>(p.out);
+  for (size_t i = part; i < head; i += parts) out[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (size_t i = tail + part; i < end; i += parts) out[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 constexpr int L_MAX_PIECES = 320;                                             // where tiles are cut: a slab for each
@@ -479,7 +480,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         else                   mbar_arrive(bar_tempty + 8 * buf);
       }
     }
-    zero_tail_rows<T>(p, blockIdx.x * (32 * EPI_WARPS) + threadIdx.x - 64, gridDim.x * (32 * EPI_WARPS));
+    zero_other_rows<T>(p, blockIdx.x * (32 * EPI_WARPS) + threadIdx.x - 64, gridDim.x * (32 * EPI_WARPS));
   }
 
   // ---- teardown ----
@@ -674,7 +675,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
       }
     }
-    zero_tail_rows<T>(p, blockIdx.x * (32 * EPI_WARPS) + threadIdx.x - 64, gridDim.x * (32 * EPI_WARPS));
+    zero_other_rows<T>(p, blockIdx.x * (32 * EPI_WARPS) + threadIdx.x - 64, gridDim.x * (32 * EPI_WARPS));
   }
 
   if (*abort_flag) {            // copies that are still in flight land before the shared memory is released

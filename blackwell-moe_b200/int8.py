@@ -2,7 +2,8 @@
 
 ``value = code * scale`` on both sides.  Weights keep the package's ``[E, in, out]`` layout, int8, with scales
 ``[E, out]`` fp32 (``quantize_expert_weights_int8`` makes them at load time); activations are quantised token by token
-on every call.  The products are summed in 32-bit integers, exactly, on the tensor cores.  Inference only: no gradients.
+on every call.  The products are summed in 32-bit integers, exactly, on the tensor cores, so a token's result does not
+depend on the batch around it.  Inference only: no gradients.
 
 The reference has no counterpart (its integer path, src/blackwell_moe/kernels/int4_moe.py, is 4-bit and weights only);
 ``int8_moe_forward`` keeps the argument order of ``fp8_moe_forward`` (src/blackwell_moe/kernels/fp8_moe.py:111-121).
@@ -92,7 +93,7 @@ def _grouped(fn_name, codes, scales, offsets, weights, w_scales, out_dtype):
 
 def int8_grouped_gemm(codes, scales, offsets, w, w_scales, out_dtype=torch.bfloat16) -> torch.Tensor:
     """``out[M,N]``: the rows ``offsets[e] .. offsets[e+1]-1`` of ``codes[M,K]`` int8 (scales ``[M]``) times ``w[e]`` of
-    ``w[E,K,N]`` int8 (scales ``[E,N]``); K and N multiples of 16.  Rows behind the last segment are zero."""
+    ``w[E,K,N]`` int8 (scales ``[E,N]``); K and N multiples of 16.  Rows of no segment are zero."""
     return _grouped("bwmoe_int_grouped_gemm", codes, scales, offsets, (w,), (w_scales,), out_dtype)
 
 

@@ -529,8 +529,9 @@ int bwmoe_unpermute_rows_backward(const void* d_dout, const void* d_rows, const 
  * ---- experts in 8-bit integers ("int"): a scale for each row of the activations and for each channel of the weights ----
  *
  * value = code * scale on both sides.  Weights [E, K, N] int8, N contiguous, channel scales [E, N] fp32.  Products are
- * summed in 32-bit integers (exact; K < 131072), scaled in fp32 and rounded once to the output type.  K and N are
- * multiples of 16, E <= 256.  No counterpart in the reference (its integer path is 4-bit, weights only).
+ * summed in 32-bit integers (exact; K < 131072), scaled in fp32 and rounded once to the output type: a row's result depends
+ * on the row and the weights only, not on the batch.  K and N are multiples of 16, E <= 256; tensors (but not the row
+ * scales) are 16-byte aligned.  Offsets past the rows are clamped.  No counterpart in the reference (its integer path is 4-bit, weights only).
  *
  * bwmoe_int_quant: scale[t] = fl32(max|x[t,:]| / 127), codes = x / scale rounded to nearest, ties to even, exactly.  A
  * row of zeros gets scale 0; a row with an infinity or a NaN gets scale NaN and codes 0, which makes its products NaN.
@@ -540,7 +541,7 @@ int bwmoe_unpermute_rows_backward(const void* d_dout, const void* d_rows, const 
 int bwmoe_int_quant(const void* d_x, const int32_t* d_pos, const int32_t* d_offsets, int T, int D, int E, int K, int dtype,
                      void* d_codes, float* d_scales, void* stream);
 /* out[m,:] = (codes[m,:] x w[e]) * row_scale[m] * channel_scale[e,:] for the rows m of segment e; d_offsets null with E = 1:
- * every row.  Rows behind the last segment are written as zeros.  dtype: of the result.
+ * every row.  Rows of no segment (in front of the first, behind the last) are written as zeros.  dtype: of the result.
  * d_scratch: bwmoe_int_scratch_bytes() bytes, 16-byte aligned; its first word is the call's status word (BWMOE_STATUS_*). */
 size_t bwmoe_int_scratch_bytes(int M, int K, int N, int E);
 int bwmoe_int_grouped_gemm(const void* d_codes, const float* d_row_scale, const int32_t* d_offsets, const void* d_w,

@@ -353,9 +353,11 @@ def test_segments_from_elsewhere_stay_inside_the_rows():
     M, K, N, E = 40, 64, 64, 3
     a, w = make_codes((M, K), 1).to(DEV), make_codes((E, K, N), 2).to(DEV)
     rs, cs = torch.ones(M, device=DEV), torch.ones(E, N, device=DEV)
-    for offsets in ([0, 10, 30, 4000], [-7, 10, 30, 40], [0, 2 ** 31 - 1, 30, 40], [40, 10, 5, 0]):
+    for offsets in ([0, 10, 30, 4000], [-7, 10, 30, 40], [0, 2 ** 31 - 1, 30, 40], [40, 40, 40, 40], [40, 10, 5, 0]):
         out = bw.int8_grouped_gemm(a, rs, torch.tensor(offsets, dtype=torch.int32, device=DEV), w, cs, out_dtype=F32)
         torch.cuda.synchronize()
+        if offsets[0] > 0:
+            assert (out == 0).all()
         if offsets[1:3] == [10, 30]:
             for e, (lo, hi) in enumerate(((0, 10), (10, 30), (30, 40))):
                 assert torch.equal(out[lo:hi].double(), a[lo:hi].double() @ w[e].double())
@@ -389,6 +391,28 @@ def test_long_products(counts, loose, K, N, swiglu):
             ref, bound = gate, gate.abs() * (3.01 * U32 + half_step(BF16) * 1.001) + smallest_step(BF16)
         assert ((out[rows].double() - ref).abs() <= bound).all(), e
     assert (out[sum(counts):] == 0).all()
+
+
+def test_a_long_matmul():
+    """Quantisation in front of a product on CTA pairs."""
+    T, K, N = 8200, 4096, 12288
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn(T, K, generator=g, device=DEV).to(BF16)
+    w, s = bw.quant_int8_channels(torch.randn(K, N, generator=g, device=DEV) * 0.02)
+    out = bw.int8_matmul(x, w, s)
+    rows = [0, 1, 127, 128, 255, 256, 4000, 8191, 8192, 8198, 8199]
+    codes, scale = (v.to(DEV) for v in exact_codes(x[rows].cpu()))
+    ref = (codes.double() @ w.double()) * scale[:, None].double() * s.double()
+    assert ((out[rows].double() - ref).abs() <= ref.abs() * (3.01 * U32 + half_step(BF16) * 1.001) + smallest_step(BF16)).all()
+
+
+def test_rows_in_front_of_the_first_segment_are_zero():
+    a, w = make_codes((300, 64), 1).to(DEV), make_codes((2, 64, 48), 2).to(DEV)
+    rs, cs = torch.ones(300, device=DEV), torch.ones(2, 48, device=DEV)
+    out = bw.int8_grouped_gemm(a, rs, torch.tensor([9, 100, 290], dtype=torch.int32, device=DEV), w, cs, out_dtype=F32)
+    assert (out[:9] == 0).all() and (out[290:] == 0).all()
+    for e, (lo, hi) in enumerate(((9, 100), (100, 290))):
+        assert torch.equal(out[lo:hi].double(), a[lo:hi].double() @ w[e].double())
 
 
 def test_quotients_of_all_pairs_of_16_bit_numbers():
