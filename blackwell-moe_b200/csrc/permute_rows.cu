@@ -72,8 +72,10 @@ permute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ x, const int
 }
 
 // R rows at a time and U pieces of each per thread: their places first, then their pieces, all requested before the first
-// is used.  Four to eight pieces in flight per thread, whatever K is (with R = 8 for two rows per token the registers that six absent
-// rows held kept half of the threads off the chip: 137 us for 16384 tokens x 2 rows of 4096, 61 us at the memory's rate).
+// is used.  Four or eight pieces in flight per thread, whatever K is: the registers that absent rows hold keep threads off the
+// chip (R = 8 for two rows per token: 137 us for 16384 tokens x 2 rows of 4096, 65 with R = 2).  More than four rows come four
+// at a time, two pieces of each (8192 tokens x 8 rows of 2048: 45 us, 49 eight at a time; 1003 x 8 rows of 2050 in fp32: 13 and
+// 17), or, where the batch is too small to hide a second round trip, eight at a time (64 x 6 rows: 1.8 us, 2.4 with four).
 // Blocks of 128 threads, and rows that are read once marked as such where many are in flight (16384 x 2 rows: 75 us with the
 // mark, 70 without; 8192 x 8 rows of 2048: 50 and 58, 20000 x 4 rows of 1024: 30 and 35; 256 threads: 4 to 7 % more).
 constexpr int kSumThreads = 128;
@@ -252,8 +254,10 @@ int run_unpermute(const void* rows, const int32_t* pos, const float* weights, in
                                  pieces, lanes, static_cast<P*>(out)));
     return (int)BWMOE_OK;
   };
-  return K <= 2 ? run(std::integral_constant<int, 2>{}) : K <= 4 ? run(std::integral_constant<int, 4>{})
-                                                                 : run(std::integral_constant<int, 8>{});
+  const bool small = n_tok <= 4 * sm_count();
+  return K <= 2            ? run(std::integral_constant<int, 2>{})
+         : K <= 4 || !small ? run(std::integral_constant<int, 4>{})
+                            : run(std::integral_constant<int, 8>{});
 }
 
 template <class T, int BYTES>
@@ -276,8 +280,11 @@ int run_unpermute_backward(const void* dout, const void* rows, const int32_t* po
                                  static_cast<P*>(drows), dweights));
     return (int)BWMOE_OK;
   };
-  return K <= 2 ? run(std::integral_constant<int, 2>{}) : K <= 4 ? run(std::integral_constant<int, 4>{})
-                                                                 : run(std::integral_constant<int, 8>{});
+  // eight rows at a time only where a piece is 16 bytes (8192 x 8 rows of 2048 in bf16: 98 us, 112 four at a time; with 8-byte
+  // pieces, 1003 x 8 rows of 2050 in fp32: 34 and 28)
+  return K <= 2                ? run(std::integral_constant<int, 2>{})
+         : K <= 4 || BYTES < 16 ? run(std::integral_constant<int, 4>{})
+                                : run(std::integral_constant<int, 8>{});
 }
 
 // fn(type tag, piece tag) for the element type and the widest piece
