@@ -68,6 +68,7 @@ struct I8Params {
   // The kernel in front is the one that quantised the rows, and it lets this one be scheduled beside it: weights, scales and
   // offsets are older than that kernel, so set-up and the first weight tiles do not wait for it.
   bool early;
+  bool sectors;             // out is aligned to 32 bytes
 };
 
 // Segment e, clamped to the rows there are: offsets are data from outside the kernel.
@@ -234,6 +235,17 @@ template <> struct Out<__nv_bfloat16> {
   }
   static __device__ __forceinline__ __nv_bfloat16 one(float v) { return __float2bfloat16_rn(v); }
 };
+// 32 bytes at a 16-byte aligned address; at once where it is aligned to 32.
+__device__ __forceinline__ void store_sector(void* p, const uint4& a, const uint4& b, bool aligned32) {
+  if (aligned32) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x),
+                 "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = a;
+    reinterpret_cast<uint4*>(p)[1] = b;
+  }
+}
 // fp32 results get the accurate exponential and division, 16-bit ones the fast forms (2^-21 against a rounding of 2^-9)
 template <class T> __device__ __forceinline__ float swiglu(float g, float u) {
   if constexpr (sizeof(T) == 4) return g / (1.0f + expf(-g)) * u;
@@ -434,43 +446,35 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         complete = last_slice(sl.arrivals + q.tile * EPI_WARPS + (warp - 2), q.slices, lane);
       }
-      const unsigned ok_rows = __ballot_sync(0xffffffffu, row_ok);
-      unsigned long long row_ptr[8];
-      group8_row_pointers(static_cast<T*>(p.out) + (size_t)row * p.N, lane, row_ptr);
-      // eight 16-byte pieces per lane at a time, exchanged so that a store writes 128 contiguous bytes of four rows
+      // A lane writes its row in whole 32-byte sectors.  (Pieces exchanged between lanes, so that a store covers 128 bytes of
+      // four rows, cost shared-memory cycles that the MMAs' operands want: 64 experts of 2048 x 1408
+      // with 768 rows each, SwiGLU: 255 -> 237 us, one product 142 -> 140)
+      T* dst = static_cast<T*>(p.out) + (size_t)row * p.N + n0;
 #pragma unroll 1
-      for (int c0 = 0; complete && c0 < COLS; c0 += 8 * PER) {
-        uint4 v[8];
+      for (int c = 0; complete && c < COLS; c += 32) {
+        uint32_t a[32], u[SWIGLU ? 32 : 4];
+        tmem_ld32(t_row + half * COLS + c, a);
+        if constexpr (SWIGLU) tmem_ld32(t_row + BN_HALF + half * COLS + c, u);
+        tmem_ld_wait();
+        if (q.slices > 1) {
+          slab_add<32>(part0, (size_t)EPI_WARPS * L_PART, q.slices, q.slice, c / 4, lane, a);
+          if constexpr (SWIGLU) slab_add<32>(part0, (size_t)EPI_WARPS * L_PART, q.slices, q.slice, (COLS + c) / 4, lane, u);
+        }
 #pragma unroll
-        for (int part = 0; part < 8 * PER / 32; ++part) {
-          const int c = c0 + part * 32;
-          uint32_t a[32], u[SWIGLU ? 32 : 4];
-          tmem_ld32(t_row + half * COLS + c, a);
-          if constexpr (SWIGLU) tmem_ld32(t_row + BN_HALF + half * COLS + c, u);
-          tmem_ld_wait();
-          if (q.slices > 1) {
-            slab_add<32>(part0, (size_t)EPI_WARPS * L_PART, q.slices, q.slice, c / 4, lane, a);
-            if constexpr (SWIGLU) slab_add<32>(part0, (size_t)EPI_WARPS * L_PART, q.slices, q.slice, (COLS + c) / 4, lane, u);
-          }
+        for (int j = 0; j < 32; j += 2 * PER) {
+          uint4 v[2];
 #pragma unroll
-          for (int j = 0; j < 32 / PER; ++j) {
+          for (int h = 0; h < 2; ++h) {
             float f[PER];
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-              const int x = j * PER + i;
+              const int x = j + h * PER + i;
               f[i] = __int2float_rn((int)a[x]) * rs * my_scale[c + x];
               if constexpr (SWIGLU) f[i] = swiglu<T>(f[i], __int2float_rn((int)u[x]) * rs * my_scale[64 + c + x]);
             }
-            v[part * (32 / PER) + j] = Out<T>::pack(f);
+            v[h] = Out<T>::pack(f);
           }
-        }
-        group8_transpose(v, lane);
-        const int col = n0 + c0 + (lane & 7) * PER;
-        if (col < p.N) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if ((ok_rows >> ((lane & ~7) + k)) & 1u)
-              *reinterpret_cast<uint4*>(static_cast<uintptr_t>(row_ptr[k]) + (size_t)col * sizeof(T)) = v[k];
+          if (row_ok && n0 + c + j < p.N) store_sector(dst + c + j, v[0], v[1], p.sectors);       // (N is a multiple of 16)
         }
       }
       tc_fence_before();
@@ -728,12 +732,13 @@ bool may_slice(int M, int n_tiles) { return (long long)ceil_div(M, BM) * n_tiles
 constexpr size_t kArrivalsAt = 16;
 constexpr size_t kSlabsAt = kArrivalsAt + (S_MAX_PIECES > L_MAX_PIECES ? S_MAX_PIECES : L_MAX_PIECES) / 2 * EPI_WARPS * sizeof(uint32_t);
 
-// CTA pairs (256-row tiles, every weight byte enters one of the two shared memories) take a third of the traffic into the SMs
-// away: an SM takes in about 64 bytes a cycle, and a 128 x 256 tile alone asks for 96 while its MMAs run.  They pay in products
-// long enough to run at the power limit; in short ones what they add at either end of a tile costs more, and with few rows
-// per expert the rows past a segment's end do.  Measured, us, pairs against single CTAs (alternating, queued back to back):
-//   8 experts, 4096 rows each:  4096 x 14336 SwiGLU 2740 / 3000,  14336 x 4096 1560 / 1660;  2048 rows each: 1390 / 1490, 705 / 760
-//   one matrix, 8192 rows:  8192 x 8192 368 / 454,  4096 x 14336 334 / 380,  1024 x 8192 100 / 82;  4096 rows, 8192 x 8192: 216 / 199
+// CTA pairs (256-row tiles, every weight byte enters one of the two shared memories).  A 128 x 256 tile reads 96 bytes of
+// operands a cycle from shared memory and wants 96 more written by its loads, of the 128 there are: the tensor pipe is busy 65 to
+// 78 % of the time.  A pair's tile needs 64 + 64 (94 %).  Pairs pay in products long enough to run at the power limit; in short
+// ones what they add at either end of a tile costs more, and with few rows per expert the rows past a segment's end do.
+// Measured, us, pairs against single CTAs (alternating, queued back to back):
+//   8 experts, 4096 rows each:  4096 x 14336 SwiGLU 2720 / 2895,  14336 x 4096 1430 / 1620;  2048 rows each: 1515 / 1545, 715 / 785
+//   one matrix, 8192 rows:  8192 x 8192 386 / 485,  4096 x 14336 372 / 412,  1024 x 8192 100 / 82;  4096 rows, 8192 x 8192: 216 / 199
 //   64 experts, 768 rows each, 2048 x 1408 SwiGLU 328 / 301;  1024 rows each of 8 x 4096 x 14336 SwiGLU 852 / 775
 constexpr int kPairMinRows = 2048;                     // per expert
 constexpr double kPairMinProducts = 4e11;
@@ -857,7 +862,8 @@ int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offse
   if (int rc = small ? make_map_rows32(&ma, a, M, K) : make_map_a(&ma, a, M, K)) return rc;
   if (int rc = make_map_b(&mb0, w0, E, K, N)) return rc;
   if (int rc = make_map_b(&mb1, swiglu ? w1 : w0, E, K, N)) return rc;
-  I8Params p{offsets, row_scale, scale0, scale1, out, status, E, M, K, N, n_tiles, early && !clear};
+  I8Params p{offsets, row_scale, scale0, scale1, out, status, E, M, K, N, n_tiles, early && !clear,
+             reinterpret_cast<uintptr_t>(out) % 32 == 0};
   if (small && narrow_applies(M, N, E, swiglu)) p.n_tiles = ceil_div(N, BN_HALF);
   uint8_t* s = static_cast<uint8_t*>(scratch);
   const bool slabs = small || may_slice(M, n_tiles);
