@@ -324,7 +324,7 @@ struct Int8Layout {
 
 bool make_int8_layout(int T, int D, int H, int E, int K, Int8Layout* L) {
   if (T <= 0 || D <= 0 || H <= 0 || E <= 0 || K <= 0 || D % 16 != 0 || H % 16 != 0 || E > 256 || K > E || K > 32) return false;
-  if ((long long)T * K >= (1ll << 31) || std::max(D, H) >= (1 << 17)) return false;
+  if ((long long)T * K > kMaxRows || std::max(D, H) >= (1 << 17)) return false;
   const size_t M = (size_t)T * K;
   size_t o = 0;
   auto take = [&](size_t bytes) {
@@ -884,6 +884,7 @@ int bwmoe_permute_tokens(const void* x, const int32_t* indices, int T, int D, in
   BWMOE_REQUIRE(x && rows, BWMOE_ERR_NULL, "permute_tokens: null pointer");
   BWMOE_REQUIRE(D > 0 && K <= 32 && dtype >= BWMOE_BF16 && dtype <= BWMOE_F32, BWMOE_ERR_UNSUPPORTED,
                 "permute_tokens: D=%d K=%d type %d", D, K, dtype);
+  BWMOE_REQUIRE((long long)T * K <= kMaxRows, BWMOE_ERR_UNSUPPORTED, "permute_tokens: T*K too large");
   BWMOE_REQUIRE((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows)) % dtype_bytes(dtype) == 0, BWMOE_ERR_BAD_ALIGN,
                 "permute_tokens: a pointer is not aligned to its type");
   if (T > 0 && E > 0 && K > 0 && D <= (1 << 20) && plan_permute_applicable(T, E, K))

@@ -76,6 +76,8 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline size_t dtype_bytes(int dtype) { return dtype == BWMOE_F32 ? 4 : 2; }
 template <class T> struct TypeTag { using type = T; };
+// Rows at most, where sizes that round up to a tile stay in 32 bits (permutation, 8-bit integers).
+constexpr long long kMaxRows = (1ll << 31) - 4096;
 int sm_count();
 int gemm_sm_budget();   // sm_count() minus the SMs reserved through bwmoe_set_sm_reserve
 

@@ -839,6 +839,7 @@ int check_int8_gemm(const void* a, const float* row_scale, const int32_t* offset
   BWMOE_REQUIRE(M > 0 && K > 0 && N > 0 && E > 0, BWMOE_ERR_BAD_SHAPE, "%s: M=%d K=%d N=%d E=%d", who, M, K, N, E);
   BWMOE_REQUIRE(K % 16 == 0 && N % 16 == 0, BWMOE_ERR_BAD_SHAPE, "%s: K=%d and N=%d must be multiples of 16", who, K, N);
   BWMOE_REQUIRE(E <= kMaxGroups, BWMOE_ERR_UNSUPPORTED, "%s: E=%d > %d", who, E, kMaxGroups);
+  BWMOE_REQUIRE(M <= kMaxRows, BWMOE_ERR_UNSUPPORTED, "%s: M=%d rows", who, M);
   BWMOE_REQUIRE(K < (1 << 17), BWMOE_ERR_UNSUPPORTED, "%s: K=%d: sums of 2^17 products or more do not fit 32 bits", who, K);
   BWMOE_REQUIRE(dtype >= BWMOE_BF16 && dtype <= BWMOE_F32, BWMOE_ERR_UNSUPPORTED, "%s: unknown type %d", who, dtype);
   BWMOE_REQUIRE(a && row_scale && w0 && scale0 && out && status && (!swiglu || scale1), BWMOE_ERR_NULL, "%s: null pointer", who);

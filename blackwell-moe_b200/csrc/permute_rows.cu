@@ -215,7 +215,7 @@ int lanes_for(int pieces, int threads) {
 int check_rows(const char* who, int T, int D, int K, int dtype) {
   BWMOE_REQUIRE(T > 0 && D > 0 && K > 0, BWMOE_ERR_BAD_SHAPE, "%s: T=%d D=%d K=%d", who, T, D, K);
   BWMOE_REQUIRE(K <= 32, BWMOE_ERR_UNSUPPORTED, "%s: K=%d > 32 slots per token", who, K);
-  BWMOE_REQUIRE((long long)T * K < (1ll << 31), BWMOE_ERR_UNSUPPORTED, "%s: T*K too large", who);
+  BWMOE_REQUIRE((long long)T * K <= kMaxRows, BWMOE_ERR_UNSUPPORTED, "%s: T*K too large", who);
   BWMOE_REQUIRE(D <= (1 << 24), BWMOE_ERR_UNSUPPORTED, "%s: D=%d too large", who, D);
   BWMOE_REQUIRE(dtype >= BWMOE_BF16 && dtype <= BWMOE_F32, BWMOE_ERR_UNSUPPORTED, "%s: unknown type %d", who, dtype);
   return BWMOE_OK;

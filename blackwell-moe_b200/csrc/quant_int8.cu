@@ -232,7 +232,7 @@ quant_int8_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ pos,
 int launch_quant_int8_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
                            void* codes, float* scales, cudaStream_t st, void* zero, size_t zero_bytes) {
   BWMOE_REQUIRE(T > 0 && D > 0 && K > 0 && D % 16 == 0, BWMOE_ERR_BAD_SHAPE, "int_quant: T=%d D=%d K=%d (D a multiple of 16)", T, D, K);
-  BWMOE_REQUIRE((long long)T * K < (1ll << 31), BWMOE_ERR_UNSUPPORTED, "int_quant: T*K too large");
+  BWMOE_REQUIRE((long long)T * K <= kMaxRows, BWMOE_ERR_UNSUPPORTED, "int_quant: T*K too large");
   BWMOE_REQUIRE(dtype >= BWMOE_BF16 && dtype <= BWMOE_F32, BWMOE_ERR_UNSUPPORTED, "int_quant: unknown type %d", dtype);
   BWMOE_REQUIRE(x && codes && scales, BWMOE_ERR_NULL, "int_quant: null pointer");
   BWMOE_REQUIRE(pos == nullptr ? K == 1 : (offsets != nullptr && E > 0), BWMOE_ERR_BAD_SHAPE,

@@ -63,6 +63,11 @@ def test_entry_points_refuse_before_any_device_work():
     assert bad(lib.bwmoe_permute_rows(p, None, p, 4, 16, 8, 2, 0, p, None), -6, "permute_rows")
     assert bad(lib.bwmoe_permute_rows(p + 2, p, p, 4, 16, 8, 2, 2, p, None), -2, "permute_rows")
     assert bad(lib.bwmoe_permute_rows(p, p, p, 2 ** 30, 16, 8, 2, 0, p, None), -4, "too large")
+    for n in (2 ** 31 - 1, 2 ** 31 - 4095):       # sizes that round up to a tile would leave 32 bits
+        assert bad(lib.bwmoe_unpermute_rows(p, p, None, n, 16, 1, 0, p, None), -4, "too large")
+        assert bad(lib.bwmoe_permute_tokens(p, p, n, 16, 8, 1, 0, p, p, p, p, p, p, p, None), -4, "too large")
+        assert bad(lib.bwmoe_int_quant(p, None, None, n, 32, 1, 1, 0, p, p, None), -4, "too large")
+        assert bad(lib.bwmoe_int_grouped_gemm(p, p, p, p, p, n, 32, 48, 2, 0, p, p, 1 << 40, None), -4, "rows")
     assert bad(lib.bwmoe_permute_tokens(p, p, 4, 16, 300, 2, 0, p, p, p, p, p, p, p, None), -4, "plan")
     assert bad(lib.bwmoe_unpermute_rows(p, p, None, 4, 0, 2, 0, p, None), -1, "unpermute_rows")
     assert bad(lib.bwmoe_unpermute_rows_backward(p, p, p, p, p, 4, 16, 8, 2, 0, None, None, None), -6, "backward")
