@@ -9,7 +9,7 @@ rounded once.  Both are differentiable (once): in the tokens and the rows, and i
 
 from __future__ import annotations
 
-from typing import NamedTuple
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -24,11 +24,12 @@ class PermutePlan(NamedTuple):
 
     ``offsets[E+1]``: expert e's rows are ``offsets[e] .. offsets[e+1]-1``; ``pos[T,K]``: the row of each slot;
     ``row_slot[M]``: the slot of each row, ``t*K + k``; ``row_expert[M]``: its expert.  A slot whose expert id is
-    outside ``[0, E)`` has no row (``pos`` -1), and the rows past ``offsets[E]`` then have no slot (-1)."""
+    outside ``[0, E)`` has no row (``pos`` -1), and the rows past ``offsets[E]`` then have no slot (-1).  The operators
+    read ``offsets`` and ``pos`` only: a plan made elsewhere may leave the other two out."""
     offsets: torch.Tensor
     pos: torch.Tensor
-    row_slot: torch.Tensor
-    row_expert: torch.Tensor
+    row_slot: Optional[torch.Tensor] = None
+    row_expert: Optional[torch.Tensor] = None
 
 
 def _dtype_code(t: torch.Tensor, name: str) -> int:

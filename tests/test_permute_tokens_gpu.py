@@ -299,7 +299,7 @@ def test_places_outside_the_rows_are_no_rows():
     """A plan made elsewhere: places past the rows or negative add nothing and are never written through."""
     T, D, K = 4, 32, 2
     pos = torch.tensor([[0, 99], [-5, 3], [2 ** 31 - 1, 1], [2, -2 ** 31]], dtype=torch.int32, device=DEV)
-    plan = bw.PermutePlan(torch.tensor([0, 8], dtype=torch.int32, device=DEV), pos, None, None)
+    plan = bw.PermutePlan(torch.tensor([0, 8], dtype=torch.int32, device=DEV), pos)
     rows = torch.randn(8, D, device=DEV)
     out = bw.unpermute_tokens(rows, plan)
     assert torch.equal(out, rows[[0, 3, 1, 2]])
