@@ -240,12 +240,49 @@ def test_block_is_its_operators_in_a_row(T, D, H, E, K, dtype, zipf):
     assert (out.double() - ref).norm() <= ref.norm() * (half_step(dtype) + 1e-3)
 
 
-def test_block_with_its_router():
-    T, D, H, E, K = 130, 256, 512, 16, 2
+@pytest.mark.parametrize("T,E,K", [(1, 8, 2), (130, 16, 2), (700, 64, 6), (2100, 8, 1)])
+def test_block_with_its_router(T, E, K):
+    D, H = 256, 512
     x, _, _, ws, ss = make_block(T, D, H, E, K, BF16, 3)
     gate = (torch.randn(D, E, device=DEV) * 0.02).to(BF16)
     out = bw.int8_moe_forward(x, gate, *ws, *ss, top_k=K)
     assert torch.equal(out, bw.int8_moe_forward_routed(x, *bw.top_k_router(x, gate, K), *ws, *ss))
+
+
+@pytest.mark.parametrize("T", [20, 1500])
+def test_status_words_and_reserved_sms(T):
+    """The C entry points: the workspace's status word tells of an expert id out of range, and of nothing else; SMs left free
+    change no result."""
+    import ctypes
+    from blackwell_moe_b200 import _lib
+    lib, stream = bw.lib(), torch.cuda.current_stream().cuda_stream
+    D, H, E, K = 256, 512, 8, 2
+    x, weights, idx, ws, ss = make_block(T, D, H, E, K, BF16, 2)
+    n = lib.bwmoe_workspace_bytes_int(T, D, H, E, K)
+    space = torch.full((n,), 0xff, dtype=torch.uint8, device=DEV)          # whatever was there before
+    status = ctypes.c_int32(-1)
+
+    def call(ids):
+        out = torch.empty_like(x)
+        _lib.check(lib.bwmoe_moe_forward_int_routed(x.data_ptr(), weights.data_ptr(), ids.data_ptr(), *[t.data_ptr() for t in ws],
+                                                    *[t.data_ptr() for t in ss], T, D, H, E, K, 0, out.data_ptr(),
+                                                    space.data_ptr(), n, stream))
+        _lib.check(lib.bwmoe_read_status(space.data_ptr(), stream, ctypes.byref(status)))
+        return out
+
+    want = call(idx)
+    assert status.value == 0
+    bad = idx.clone()
+    bad[7, 1] = E
+    call(bad)
+    assert status.value == 2
+    for reserve in (100, 127):
+        assert lib.bwmoe_set_sm_reserve(reserve) == 0
+        try:
+            got = call(idx)
+        finally:
+            lib.bwmoe_set_sm_reserve(0)
+        assert status.value == 0 and torch.equal(got, want)
 
 
 def test_block_beside_the_reference_in_bf16():
