@@ -11,6 +11,8 @@ The reference has no counterpart (its integer path, src/blackwell_moe/kernels/in
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -102,6 +104,11 @@ def int8_grouped_swiglu(codes, scales, offsets, w_gate, w_up, s_gate, s_up, out_
     return _grouped("bwmoe_int_gateup_swiglu", codes, scales, offsets, (w_gate, w_up), (s_gate, s_up), out_dtype)
 
 
+@functools.lru_cache(maxsize=256)
+def _matmul_workspace_bytes(device_index, T, K, N):         # (sizes go by the device's SMs)
+    return _lib.lib().bwmoe_workspace_bytes_int_matmul(T, K, N)
+
+
 def int8_matmul(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
     """``x[T,K]`` (bf16, fp16 or fp32), quantised token by token, times ``w[K,N]`` int8 with scales ``[N]``, in x's type."""
     assert x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[0], (x.shape, w.shape)
@@ -114,7 +121,7 @@ def int8_matmul(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor) -> tor
         return out
     lib = _lib.lib()
     with _on_device(dev):
-        need = lib.bwmoe_workspace_bytes_int_matmul(T, K, N)
+        need = _matmul_workspace_bytes(dev.index, T, K, N)
         if need == 0:
             raise ValueError(f"unsupported shape T={T} K={K} N={N} (K and N must be multiples of 16)")
         ws = _call_workspace(dev, need)

@@ -9,6 +9,7 @@ rounded once.  Both are differentiable (once): in the tokens and the rows, and i
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -39,6 +40,11 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
+@functools.lru_cache(maxsize=256)
+def _plan_scratch_bytes(T, num_experts, K):
+    return _lib.lib().bwmoe_plan_scratch_bytes(T, num_experts, K)
+
+
 def _empty_plan(indices, T, K, num_experts, scratch_bytes):
     """The plan's tensors, and the addresses of its status word and scratch behind them: one allocation."""
     M, extra = T * K, 4 + (scratch_bytes + 3) // 4
@@ -64,6 +70,12 @@ def _check_plan(plan, name="plan"):
     return offsets, pos
 
 
+def _elsewhere(dev):
+    """Whether a call has to make its tensors' device the current one first.  (The usual answer costs a tenth of a context
+    manager, and small batches are bound by the host.)"""
+    return dev.index != torch.cuda.current_device()
+
+
 def permute_plan(indices: torch.Tensor, num_experts: int) -> PermutePlan:
     """The stable sort of all slots of ``indices[T,K]`` int32 by expert id."""
     indices = _check_indices(indices, num_experts)
@@ -71,7 +83,7 @@ def permute_plan(indices: torch.Tensor, num_experts: int) -> PermutePlan:
     T, K = indices.shape
     lib = _lib.lib()
     with _on_device(dev):
-        plan, status, scratch = _empty_plan(indices, T, K, num_experts, lib.bwmoe_plan_scratch_bytes(T, num_experts, K))
+        plan, status, scratch = _empty_plan(indices, T, K, num_experts, _plan_scratch_bytes(T, num_experts, K))
         if T == 0:
             plan.offsets.zero_()
             return plan
@@ -83,41 +95,46 @@ def permute_plan(indices: torch.Tensor, num_experts: int) -> PermutePlan:
 
 def _permute_new(x, indices, num_experts):
     """The plan and the rows in one call."""
-    T, K = indices.shape
-    D, dev = x.shape[1], x.device
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _permute_new(x, indices, num_experts)
+    (T, K), D = indices.shape, x.shape[1]
     lib = _lib.lib()
-    with _on_device(dev):
-        plan, status, scratch = _empty_plan(indices, T, K, num_experts, lib.bwmoe_plan_scratch_bytes(T, num_experts, K))
-        rows = x.new_empty((T * K, D))
-        pos = plan.pos.data_ptr()
-        _lib.check(lib.bwmoe_permute_tokens(x.data_ptr(), indices.data_ptr(), T, D, num_experts, K, _DTYPES[x.dtype],
-                                            plan.offsets.data_ptr(), pos, pos + 4 * T * K, pos + 8 * T * K, rows.data_ptr(),
-                                            status, scratch, _stream(dev)))
+    plan, status, scratch = _empty_plan(indices, T, K, num_experts, _plan_scratch_bytes(T, num_experts, K))
+    rows = x.new_empty((T * K, D))
+    pos = plan.pos.data_ptr()
+    _lib.check(lib.bwmoe_permute_tokens(x.data_ptr(), indices.data_ptr(), T, D, num_experts, K, _DTYPES[x.dtype],
+                                        plan.offsets.data_ptr(), pos, pos + 4 * T * K, pos + 8 * T * K, rows.data_ptr(),
+                                        status, scratch, _stream(dev)))
     return rows, plan
 
 
 def _permute(x, offsets, pos):
     """rows[pos[t,k]] = x[t]"""
-    T, K = pos.shape
-    D, dev = x.shape[1], x.device
-    with _on_device(dev):
-        rows = x.new_empty((T * K, D))
-        if T and D:
-            _lib.check(_lib.lib().bwmoe_permute_rows(x.data_ptr(), pos.data_ptr(), offsets.data_ptr(), T, D, offsets.numel() - 1,
-                                                     K, _DTYPES[x.dtype], rows.data_ptr(), _stream(dev)))
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _permute(x, offsets, pos)
+    (T, K), D = pos.shape, x.shape[1]
+    rows = x.new_empty((T * K, D))
+    if T and D:
+        _lib.check(_lib.lib().bwmoe_permute_rows(x.data_ptr(), pos.data_ptr(), offsets.data_ptr(), T, D, offsets.numel() - 1,
+                                                 K, _DTYPES[x.dtype], rows.data_ptr(), _stream(dev)))
     return rows
 
 
 def _unpermute(rows, pos, weights):
     """sum over k of w[t,k] * rows[pos[t,k]]"""
-    T, K = pos.shape
-    D, dev = rows.shape[1], rows.device
-    with _on_device(dev):
-        out = rows.new_empty((T, D))
-        if T and D:
-            _lib.check(_lib.lib().bwmoe_unpermute_rows(rows.data_ptr(), pos.data_ptr(),
-                                                       None if weights is None else weights.data_ptr(), T, D, K,
-                                                       _DTYPES[rows.dtype], out.data_ptr(), _stream(dev)))
+    dev = rows.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _unpermute(rows, pos, weights)
+    (T, K), D = pos.shape, rows.shape[1]
+    out = rows.new_empty((T, D))
+    if T and D:
+        _lib.check(_lib.lib().bwmoe_unpermute_rows(rows.data_ptr(), pos.data_ptr(), None if weights is None else weights.data_ptr(),
+                                                   T, D, K, _DTYPES[rows.dtype], out.data_ptr(), _stream(dev)))
     return out
 
 
@@ -219,11 +236,12 @@ def _check_unpermute(rows, plan, weights):
     _dtype_code(rows, "rows")
     offsets, pos = _check_plan(plan)
     assert rows.shape[0] == pos.numel(), (rows.shape, pos.shape)
-    tensors = [_contig(rows, "rows"), offsets, pos]
-    if weights is not None:
+    _contig(rows, "rows")
+    if weights is None:
+        _require_cuda(rows, offsets, pos)
+    else:
         assert weights.shape == pos.shape and weights.dtype == torch.float32, (weights.shape, weights.dtype)
-        tensors.append(_contig(weights, "weights"))
-    _require_cuda(*tensors)
+        _require_cuda(rows, offsets, pos, _contig(weights, "weights"))
     return offsets, pos
 
 
