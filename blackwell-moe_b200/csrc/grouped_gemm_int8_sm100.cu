@@ -734,17 +734,20 @@ constexpr size_t kSlabsAt = kArrivalsAt + (S_MAX_PIECES > L_MAX_PIECES ? S_MAX_P
 
 // CTA pairs (256-row tiles, every weight byte enters one of the two shared memories).  A 128 x 256 tile reads 96 bytes of
 // operands a cycle from shared memory and wants 96 more written by its loads, of the 128 there are: the tensor pipe is busy 65 to
-// 78 % of the time.  A pair's tile needs 64 + 64 (94 %).  Pairs pay in products long enough to run at the power limit; in short
-// ones what they add at either end of a tile costs more, and with few rows per expert the rows past a segment's end do.
-// Measured, us, pairs against single CTAs (alternating, queued back to back):
-//   8 experts, 4096 rows each:  4096 x 14336 SwiGLU 2720 / 2895,  14336 x 4096 1430 / 1620;  2048 rows each: 1515 / 1545, 715 / 785
-//   one matrix, 8192 rows:  8192 x 8192 386 / 485,  4096 x 14336 372 / 412,  1024 x 8192 100 / 82;  4096 rows, 8192 x 8192: 216 / 199
-//   64 experts, 768 rows each, 2048 x 1408 SwiGLU 328 / 301;  1024 rows each of 8 x 4096 x 14336 SwiGLU 852 / 775
-constexpr int kPairMinRows = 2048;                     // per expert
-constexpr double kPairMinProducts = 4e11;
+// 78 % of the time.  A pair's tile needs 64 + 64 (94 %).  Against it: the rows past a segment's end (half a tile on average, 128
+// instead of 64), a start across two SMs, and with SwiGLU an epilogue that keeps up with fewer of a pair's MMAs.  Measured, us,
+// pairs / single CTAs (alternating, queued back to back):
+//   one product, one matrix:  8192 rows, 8192 x 8192 349 / 449, 2048 x 8192 95 / 105, 1024 x 8192 67 / 67, 512 x 8192 59 / 56;
+//     4096 rows, 4096 x 4096 50.5 / 56.3;  2048 rows, 8192 x 8192 92.5 / 98.6;  1024 rows, 4096 x 4096 (64 tiles) 25.7 / 22.1
+//   one product, 64 experts:  768 rows each, 2048 x 1536 138 / 149, 1408 x 2048 149 / 155;  1024 rows, 173 / 190, 201 / 196
+//   one product, 8 experts of 14336 x 4096:  512 rows each 244 / 208, 1024 rows 356 / 391, 4096 rows 1430 / 1620
+//   SwiGLU:  8 experts of 4096 x 14336, 1024 rows each 800 / 783, 2048 rows 1460 / 1490, 4096 rows 2720 / 2895;
+//     64 experts of 2048 x 1408, 1024 rows each 359 / 336, 2048 rows 580 / 624
 bool pair_applies(int M, int K, int N, int E, bool swiglu) {
-  return (long long)M >= (long long)kPairMinRows * E && (double)M * K * N * (swiglu ? 2 : 1) >= kPairMinProducts &&
-         (swiglu || N % BN == 0) && gemm_sm_budget() >= 2;
+  if (gemm_sm_budget() < 2) return false;
+  if (swiglu) return M >= 2048ll * E && 2.0 * M * K * N >= 4e11;
+  const long long tiles = (long long)(M / (2 * BM)) * (N / BN);
+  return M >= 768ll * E && K >= 1408 && N % BN == 0 && tiles >= 3 * (sm_count() / 2);
 }
 
 template <class Kernel>

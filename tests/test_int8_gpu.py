@@ -401,7 +401,8 @@ def test_segments_from_elsewhere_stay_inside_the_rows():
 
 
 @pytest.mark.parametrize("swiglu", [False, True])
-@pytest.mark.parametrize("counts,loose,K,N", [([5000, 4000], 7, 4096, 8192), ([8200], 0, 8192, 6144), ([0, 3001, 257, 9000, 1], 300, 4096, 7680)])
+@pytest.mark.parametrize("counts,loose,K,N", [([5000, 4000], 7, 4096, 8192), ([8200], 0, 8192, 6144), ([0, 3001, 257, 9000, 1], 300, 4096, 7680),
+                                                ([900, 1, 0, 2500, 700, 1111, 890, 1500], 5, 1408, 8192)])
 def test_long_products(counts, loose, K, N, swiglu):
     """Products long enough for CTA pairs, with segments that end anywhere in a pair's tile; some rows are compared."""
     M, E = sum(counts) + loose, len(counts)
