@@ -12,21 +12,27 @@ The reference has no counterpart (its integer path, src/blackwell_moe/kernels/in
 from __future__ import annotations
 
 import functools
+import threading
 
 import torch
 
 from . import _lib
-from .moe import _contig, _on_device, _require_cuda, _stream, _workspace
+from .moe import _contig, _on_device, _require_cuda, _stream, _workspaces
 from .permute import _DTYPES, _check_plan, _dtype_code
 
 _I8 = torch.int8
 
 
 def _call_workspace(dev, nbytes: int) -> torch.Tensor:
-    """The stream's workspace; during capture one of the graph's own, so that graphs replayed side by side share nothing."""
+    """The workspace of this thread's calls on this stream (a call is several launches, and two threads' launches may
+    interleave); during capture one of the graph's own, so that graphs replayed side by side share nothing."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return _workspace(dev, nbytes)
+    key = (dev.index, _stream(dev), threading.get_ident())
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws
 
 
 def _out_code(dtype) -> int:

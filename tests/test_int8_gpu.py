@@ -370,6 +370,25 @@ def test_two_streams_at_once():
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_two_threads_on_one_stream():
+    """Calls are several launches: those of two threads interleave on the stream, and their workspaces must not be one."""
+    import threading
+    sets = [make_block(T, 512, 1024, 8, 2, BF16, T) for T in (5, 90)]
+    call = lambda s: (bw.int8_moe_forward_routed(*s[:3], *s[3], *s[4]), bw.int8_matmul(s[0], s[3][0][0], s[4][0][0]))      # noqa: E731
+    want = [call(s) for s in sets]
+    torch.cuda.synchronize()
+    got, threads = [[], []], []
+    for i, s in enumerate(sets):
+        threads.append(threading.Thread(target=lambda i=i, s=s: [got[i].append(call(s)) for _ in range(150)]))
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for outs, ref in zip(got, want):
+        assert len(outs) == 150 and all(torch.equal(a, b) for out in outs for a, b in zip(out, ref))
+
+
 def test_the_same_workspace_for_batches_of_all_sizes():
     """The stream's workspace carries what the call before left in it: sizes up and down, cut tiles and uncut ones."""
     D, H, E, K = 512, 2048, 8, 2
