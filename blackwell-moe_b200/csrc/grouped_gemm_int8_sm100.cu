@@ -77,6 +77,9 @@ __device__ __forceinline__ void segment(const I8Params& p, int e, int& r0, int& 
   r1 = p.offsets != nullptr ? min(max(p.offsets[e + 1], r0), p.M) : p.M;
 }
 
+// Segments in order have fewer tiles (the host checks); overlapping ones might not, and their count ends here.
+constexpr unsigned kMostTiles = 0x7fffffffu;
+
 // first / end: the segments; cum: tiles before each.  All threads of the block; read behind the next __syncthreads().
 template <int THREADS>
 __device__ __forceinline__ void tile_table(const I8Params& p, int tile_rows, int tiles_per_row_block, int* s_first, int* s_end,
@@ -85,25 +88,23 @@ __device__ __forceinline__ void tile_table(const I8Params& p, int tile_rows, int
     int r0 = 0, r1 = 0;
     if (e < p.E) segment(p, e, r0, r1);
     s_first[e] = r0, s_end[e] = r1;
-    // (no result that fits the memory has 2^22 tiles; segments that overlap might, and the sum over them fits 32 bits so)
-    s_cum[e + 1] = (int)min((long long)((r1 - r0 + tile_rows - 1) / tile_rows) * tiles_per_row_block, 1ll << 22);
+    s_cum[e + 1] = (int)min((long long)((r1 - r0 + tile_rows - 1) / tile_rows) * tiles_per_row_block, (long long)kMostTiles);
   }
   __syncthreads();
   if (threadIdx.x < 32) {       // inclusive scan: 8 values per lane, then a shuffle scan of the lanes' totals
     const int lane = threadIdx.x;
+    auto sum = [](int a, int b) { return (int)min((unsigned)a + (unsigned)b, kMostTiles); };
     int v[8], run = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      run += s_cum[1 + lane * 8 + j];
-      v[j] = run;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = run = sum(run, s_cum[1 + lane * 8 + j]);
     int incl = run;
     for (int off = 1; off < 32; off <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += o;
+      if (lane >= off) incl = sum(incl, o);
     }
+    const int before = __shfl_up_sync(0xffffffffu, incl, 1);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s_cum[1 + lane * 8 + j] = incl - run + v[j];
+    for (int j = 0; j < 8; ++j) s_cum[1 + lane * 8 + j] = lane > 0 ? sum(before, v[j]) : v[j];
     if (lane == 0) s_cum[0] = 0;
   }
 }
@@ -849,7 +850,8 @@ int check_int8_gemm(const void* a, const float* row_scale, const int32_t* offset
   BWMOE_REQUIRE(offsets != nullptr || E == 1, BWMOE_ERR_NULL, "%s: %d experts need offsets", who, E);
   BWMOE_REQUIRE(aligned16(a) && aligned16(w0) && aligned16(w1) && aligned16(scale0) && aligned16(scale1) && aligned16(out),
                 BWMOE_ERR_BAD_ALIGN, "%s: codes, channel scales and the result must be 16-byte aligned", who);
-  BWMOE_REQUIRE((long long)(ceil_div(M, BM) + E) * ceil_div(N, BN_HALF) < (1ll << 31), BWMOE_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  // (32-row tiles where M <= 32 E: at most 2 E of them over the rows)
+  BWMOE_REQUIRE((ceil_div(M, BM) + 2ll * E) * ceil_div(N, BN_HALF) < kMostTiles, BWMOE_ERR_UNSUPPORTED, "%s: too many tiles", who);
   return BWMOE_OK;
 }
 

@@ -485,3 +485,24 @@ def test_quotients_of_all_pairs_of_16_bit_numbers():
         for scale in (1.0, 2.0 ** -9):
             y = (x * scale).to(dtype)
             assert_codes(*bw.quantize_tokens_int8(y.to(DEV)), y)
+
+
+def test_more_tiles_than_22_bits_count():
+    """More than 2^22 tiles of 128 short rows: the ones at the end, too."""
+    M, K, N = 2 ** 29 + 40000, 16, 16
+    codes = torch.zeros(M, K, dtype=I8, device=DEV)
+    w = make_codes((1, K, N), 2).to(DEV)
+    rs, cs = torch.ones(M, device=DEV), torch.ones(1, N, device=DEV)
+    places = [slice(0, 300), slice(2 ** 28 - 200, 2 ** 28 + 200), slice(2 ** 29 - 200, 2 ** 29 + 200), slice(M - 300, M)]
+    for i, rows in enumerate(places):
+        codes[rows] = make_codes((rows.stop - rows.start, K), 3 + i).to(DEV)
+    for offsets in ([0, M], [0, M - 7]):
+        out = bw.int8_grouped_gemm(codes, rs, torch.tensor(offsets, dtype=torch.int32, device=DEV), w, cs, out_dtype=F32)
+        for rows in places:
+            want = codes[rows].double() @ w[0].double()
+            if rows.stop > offsets[1]:
+                want[offsets[1] - rows.start:] = 0
+            assert torch.equal(out[rows].double(), want), (offsets, rows)
+        assert int(torch.count_nonzero(out[300:2 ** 28 - 200])) + int(torch.count_nonzero(out[2 ** 29 + 200:M - 300])) == 0
+        del out
+    torch.cuda.empty_cache()
