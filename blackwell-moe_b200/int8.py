@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from .moe import _contig, _on_device, _require_cuda, _stream, _workspaces
-from .permute import _DTYPES, _check_plan, _dtype_code
+from .permute import _DTYPES, _MAX_SIZE, _check_plan, _check_sizes, _dtype_code
 
 _I8 = torch.int8
 
@@ -80,6 +80,7 @@ def _check_grouped(codes, scales, offsets, weights, w_scales):
     for w, s in zip(weights, w_scales):
         assert tuple(w.shape) == (E, D, N) and w.dtype == _I8, (w.shape, w.dtype)
         assert tuple(s.shape) == (E, N) and s.dtype == torch.float32, (s.shape, s.dtype)
+    _check_sizes("codes and weights", M, D, N, E)
     names = ["codes", "scales", "offsets"] + ["weights"] * len(weights) + ["weight scales"] * len(w_scales)
     dev = _require_cuda(*[_contig(t, n) for t, n in zip([codes, scales, offsets, *weights, *w_scales], names)])
     return dev, M, D, N, E
@@ -120,6 +121,7 @@ def int8_matmul(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor) -> tor
     assert x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[0], (x.shape, w.shape)
     assert w.dtype == _I8 and w_scales.dtype == torch.float32 and w_scales.shape == (w.shape[1],), (w.dtype, w_scales.shape)
     code = _dtype_code(x, "x")
+    _check_sizes("w", *w.shape)
     dev = _require_cuda(_contig(x, "x"), _contig(w, "w"), _contig(w_scales, "w_scales"))
     (T, K), N = x.shape, w.shape[1]
     out = x.new_empty((T, N))
@@ -146,12 +148,13 @@ def _check_int8_experts(x, w_gate, w_up, w_down, s_gate, s_up, s_down):
         assert w.dtype == _I8, w.dtype
     for s, n in ((s_gate, H), (s_up, H), (s_down, D)):
         assert tuple(s.shape) == (E, n) and s.dtype == torch.float32, (s.shape, s.dtype)
+    _check_sizes("x and weights", T, D, H, E)
     tensors = [_contig(t, "tensor") for t in (x, w_gate, w_up, w_down, s_gate, s_up, s_down)]
     return _require_cuda(*tensors), T, D, H, E
 
 
 def _int8_workspace(lib, dev, T, D, H, E, K):
-    need = lib.bwmoe_workspace_bytes_int(T, D, H, E, K)
+    need = lib.bwmoe_workspace_bytes_int(T, D, H, E, min(K, _MAX_SIZE))
     if need == 0:
         raise ValueError(f"unsupported shape T={T} D={D} H={H} E={E} top_k={K} "
                          "(D and H must be multiples of 16, E <= 256, top_k <= min(E, 32))")

@@ -33,7 +33,16 @@ class PermutePlan(NamedTuple):
     row_expert: Optional[torch.Tensor] = None
 
 
+_MAX_SIZE = 2 ** 31 - 4096      # sizes reach the library as 32-bit integers: a larger one would wrap on the way
+
+
+def _check_sizes(name, *sizes):
+    if max(sizes) > _MAX_SIZE:
+        raise ValueError(f"{name}: sizes {sizes}, at most {_MAX_SIZE} each")
+
+
 def _dtype_code(t: torch.Tensor, name: str) -> int:
+    _check_sizes(name, *t.shape)
     code = _DTYPES.get(t.dtype)
     if code is None:
         raise ValueError(f"{name}: {t.dtype} is not one of bfloat16, float16, float32")
@@ -59,6 +68,7 @@ def _check_indices(indices, num_experts):
     assert indices.dtype == torch.int32, indices.dtype
     if not 1 <= num_experts <= 256 or indices.shape[1] > 32:
         raise ValueError(f"{num_experts} experts and {indices.shape[1]} slots per token: at most 256 and 32")
+    _check_sizes("indices", indices.numel())
     return _contig(indices, "indices")
 
 
@@ -66,6 +76,7 @@ def _check_plan(plan, name="plan"):
     offsets, pos = plan[0], plan[1]
     assert pos.dim() == 2 and offsets.dim() == 1 and offsets.numel() >= 2, (name, pos.shape, offsets.shape)
     assert pos.dtype == torch.int32 and offsets.dtype == torch.int32, (name, pos.dtype, offsets.dtype)
+    _check_sizes(name, pos.numel(), offsets.numel())
     _contig(pos, "plan.pos"), _contig(offsets, "plan.offsets")
     return offsets, pos
 

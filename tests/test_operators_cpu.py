@@ -106,3 +106,21 @@ def test_weights_in_8_bit_integers():
     assert (err <= scales[:, None].double() * (0.5 + 127 * 2.0 ** -23)).all()       # half a step, and the quotient's rounding
     live = scales > 0
     assert (codes.abs().amax(1)[live] == 127).all()
+
+
+def test_sizes_past_32_bits_are_refused():
+    """They would reach the library modulo 2^32."""
+    big, m = 2 ** 32 + 16, lambda *shape, dtype=BF16: torch.empty(shape, dtype=dtype, device="meta")      # noqa: E731
+    plan = lambda T, K, E=8: bw.PermutePlan(m(E + 1, dtype=I32), m(T, K, dtype=I32))                       # noqa: E731
+    w, ws = m(2, 16, big, dtype=I8), m(2, big, dtype=F32)
+    for call in (lambda: bw.permute_tokens(m(big, 1), m(big, 1, dtype=I32), 8), lambda: bw.permute_tokens(m(1, big), m(1, 1, dtype=I32), 8),
+                 lambda: bw.permute_plan(m(big, 1, dtype=I32), 8), lambda: bw.permute_tokens(m(1, 16), plan=plan(1, big)),
+                 lambda: bw.permute_tokens(m(1, 16), plan=plan(1, 2, big)), lambda: bw.unpermute_tokens(m(big, 16), plan(big, 1)),
+                 lambda: bw.unpermute_tokens_backward(m(1, big), m(2, big), plan(1, 2), m(1, 2, dtype=F32)),
+                 lambda: bw.quantize_tokens_int8(m(big, 16)), lambda: bw.int8_matmul(m(1, 16), m(16, big, dtype=I8), m(big, dtype=F32)),
+                 lambda: bw.int8_grouped_gemm(m(4, 16, dtype=I8), m(4, dtype=F32), m(3, dtype=I32), w, ws),
+                 lambda: bw.int8_grouped_swiglu(m(big, 16, dtype=I8), m(big, dtype=F32), m(3, dtype=I32), *[m(2, 16, 16, dtype=I8)] * 2, *[m(2, 16, dtype=F32)] * 2),
+                 lambda: bw.int8_moe_forward(m(4, 16), m(16, 2), w, w, m(2, big, 16, dtype=I8), ws, ws, m(2, 16, dtype=F32)),
+                 lambda: bw.int8_moe_forward_routed(m(4, 16), m(4, 2, dtype=F32), m(4, 2, dtype=I32), w, w, m(2, big, 16, dtype=I8), ws, ws, m(2, 16, dtype=F32))):
+        with pytest.raises(ValueError, match="sizes"):
+            call()
