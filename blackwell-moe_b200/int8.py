@@ -12,27 +12,14 @@ The reference has no counterpart (its integer path, src/blackwell_moe/kernels/in
 from __future__ import annotations
 
 import functools
-import threading
 
 import torch
 
 from . import _lib
-from .moe import _contig, _on_device, _require_cuda, _stream, _workspaces
+from .moe import _contig, _on_device, _require_cuda, _stream, _thread_workspace
 from .permute import _DTYPES, _MAX_SIZE, _check_plan, _check_sizes, _dtype_code
 
 _I8 = torch.int8
-
-
-def _call_workspace(dev, nbytes: int) -> torch.Tensor:
-    """The workspace of this thread's calls on this stream (a call is several launches, and two threads' launches may
-    interleave); during capture one of the graph's own, so that graphs replayed side by side share nothing."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    key = (dev.index, _stream(dev), threading.get_ident())
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = _workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return ws
 
 
 def _out_code(dtype) -> int:
@@ -93,7 +80,7 @@ def _grouped(fn_name, codes, scales, offsets, weights, w_scales, out_dtype):
     if M:
         lib = _lib.lib()
         with _on_device(dev):
-            ws = _call_workspace(dev, lib.bwmoe_int_scratch_bytes(M, D, N, E))
+            ws = _thread_workspace(dev, lib.bwmoe_int_scratch_bytes(M, D, N, E))
             _lib.check(getattr(lib, fn_name)(codes.data_ptr(), scales.data_ptr(), offsets.data_ptr(),
                                              *[w.data_ptr() for w in weights], *[s.data_ptr() for s in w_scales], M, D, N, E,
                                              code, out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)))
@@ -132,7 +119,7 @@ def int8_matmul(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor) -> tor
         need = _matmul_workspace_bytes(dev.index, T, K, N)
         if need == 0:
             raise ValueError(f"unsupported shape T={T} K={K} N={N} (K and N must be multiples of 16)")
-        ws = _call_workspace(dev, need)
+        ws = _thread_workspace(dev, need)
         _lib.check(lib.bwmoe_int_matmul(x.data_ptr(), w.data_ptr(), w_scales.data_ptr(), T, K, N, code, out.data_ptr(),
                                         ws.data_ptr(), ws.numel(), _stream(dev)))
     return out
@@ -158,7 +145,7 @@ def _int8_workspace(lib, dev, T, D, H, E, K):
     if need == 0:
         raise ValueError(f"unsupported shape T={T} D={D} H={H} E={E} top_k={K} "
                          "(D and H must be multiples of 16, E <= 256, top_k <= min(E, 32))")
-    return _call_workspace(dev, need)
+    return _thread_workspace(dev, need)
 
 
 def int8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, experts_w_up, experts_w_down,

@@ -11,6 +11,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import threading
+import weakref
 
 import torch
 
@@ -67,8 +69,38 @@ def _workspace(dev, nbytes: int) -> torch.Tensor:
     return ws
 
 
+class _Workspaces:
+    def __init__(self):
+        self.by_stream: dict = {}
+
+
+class _ThreadWorkspaces(threading.local):
+    """Workspaces of one thread, by (device, stream); they go when the thread ends."""
+    def __init__(self):
+        self.mine = _Workspaces()
+        _of_threads.add(self.mine)
+
+
+_of_threads: "weakref.WeakSet[_Workspaces]" = weakref.WeakSet()
+_thread_workspaces = _ThreadWorkspaces()
+
+
+def _thread_workspace(dev, nbytes: int) -> torch.Tensor:
+    """The workspace of this thread's calls on this stream, for calls that are several launches: two threads' launches may
+    interleave.  During capture one of the graph's own, so that graphs replayed side by side share nothing."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    mine, key = _thread_workspaces.mine.by_stream, (dev.index, _stream(dev))
+    ws = mine.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = mine[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws
+
+
 def release_workspaces() -> None:
     _workspaces.clear()
+    for of_thread in list(_of_threads):
+        of_thread.by_stream.clear()
 
 
 def top_k_router(hidden: torch.Tensor, gate_w: torch.Tensor, k: int, *, as_batch: int = None):

@@ -389,6 +389,33 @@ def test_two_threads_on_one_stream():
         assert len(outs) == 150 and all(torch.equal(a, b) for out in outs for a, b in zip(out, ref))
 
 
+def test_workspaces_go_with_their_thread():
+    import threading
+    w, s = bw.quant_int8_channels(torch.randn(2048, 4096, device=DEV))
+    x = torch.randn(3, 2048, device=DEV).to(BF16)
+    want = bw.int8_matmul(x, w, s)
+    torch.cuda.synchronize()
+    before, together, same = torch.cuda.memory_allocated(), threading.Barrier(4, timeout=60), []
+    kept = []
+
+    def work():
+        same.append(bool(torch.equal(bw.int8_matmul(x, w, s), want)))
+        together.wait()                          # all live at once: every one has its own
+        kept.append(torch.cuda.memory_allocated())
+        together.wait()
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == [True] * 4 and min(kept) >= before + 4 * bw.lib().bwmoe_workspace_bytes_int_matmul(3, 2048, 4096)
+    assert torch.cuda.memory_allocated() == before
+    bw.moe.release_workspaces()
+    assert torch.cuda.memory_allocated() < before
+    assert torch.equal(bw.int8_matmul(x, w, s), want)
+
+
 def test_the_same_workspace_for_batches_of_all_sizes():
     """The stream's workspace carries what the call before left in it: sizes up and down, cut tiles and uncut ones."""
     D, H, E, K = 512, 2048, 8, 2
