@@ -42,7 +42,8 @@ def _check_sizes(name, *sizes):
 
 
 def _dtype_code(t: torch.Tensor, name: str) -> int:
-    _check_sizes(name, *t.shape)
+    if t.numel() > _MAX_SIZE:        # (a size that large, or only their product)
+        _check_sizes(name, *t.shape)
     code = _DTYPES.get(t.dtype)
     if code is None:
         raise ValueError(f"{name}: {t.dtype} is not one of bfloat16, float16, float32")
@@ -76,7 +77,8 @@ def _check_plan(plan, name="plan"):
     offsets, pos = plan[0], plan[1]
     assert pos.dim() == 2 and offsets.dim() == 1 and offsets.numel() >= 2, (name, pos.shape, offsets.shape)
     assert pos.dtype == torch.int32 and offsets.dtype == torch.int32, (name, pos.dtype, offsets.dtype)
-    _check_sizes(name, pos.numel(), offsets.numel())
+    if pos.numel() > _MAX_SIZE or offsets.numel() > _MAX_SIZE:
+        _check_sizes(name, pos.numel(), offsets.numel())
     _contig(pos, "plan.pos"), _contig(offsets, "plan.offsets")
     return offsets, pos
 
