@@ -5,7 +5,7 @@
 //
 // where e is the expert whose segment offsets[e] .. offsets[e+1] holds row m.  The sums are formed in 32-bit integers and
 // are exact whatever their order (|a|, |w| <= 128 and K < 2^17); scales, SwiGLU and the one rounding to the output type
-// happen in fp32 in the epilogue.
+// happen in fp32 in the epilogue (scaled() says in which order).
 //
 // Two kernels, persistent, one CTA per SM, warp-specialised (TMA producer, tcgen05.mma kind::i8 issuer, epilogue warps);
 // activations are read K-major, weights in the caller's [E, K, N] layout (N contiguous):
@@ -247,6 +247,19 @@ __device__ __forceinline__ void store_sector(void* p, const uint4& a, const uint
     reinterpret_cast<uint4*>(p)[1] = b;
   }
 }
+// acc * channel * row in the order that ends in infinity only where the product itself does: |acc| < 2^31, so a factor of up
+// to 2^96 can come first, and where that is the row's scale and not the channel's, the row's does.  (With both above it, any
+// acc but 0 gives infinity.)  Nothing is lost at the other end: |acc| >= 1, so acc * scale is below the normal numbers only
+// where the scale is, and then it is exact.
+constexpr float kFirstScale = 7.922816251426434e28f;      // 2^96
+__device__ __forceinline__ float scaled(uint32_t acc, float channel, float row) {
+  return __int2float_rn((int)acc) * channel * row;
+}
+__device__ __forceinline__ float scaled_any(uint32_t acc, float channel, float row) {
+  const bool row_first = channel > kFirstScale && row <= kFirstScale;
+  return scaled(acc, row_first ? row : channel, row_first ? channel : row);
+}
+
 // fp32 results get the accurate exponential and division, 16-bit ones the fast forms (2^-21 against a rounding of 2^-9)
 template <class T> __device__ __forceinline__ float swiglu(float g, float u) {
   if constexpr (sizeof(T) == 4) return g / (1.0f + expf(-g)) * u;
@@ -413,13 +426,15 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const float rs = row_ok ? p.row_scale[row] : 0.f;
       // channel scales of this warp's columns (SWIGLU: 64 of the gate, then 64 of the up product), zero past N
       const int n0 = q.n_idx * (SWIGLU ? BN_HALF : BN) + half * (SWIGLU ? BN_HALF / 2 : BN_HALF);
+      bool huge;                                 // a channel scale that may have to come second
       {
         const float* s = (SWIGLU && lane >= 16 ? p.scale1 : p.scale0) + (size_t)q.e * p.N;
         const int n = n0 + (SWIGLU ? (lane & 15) : lane) * 4;
         __syncwarp();                            // the tile before has read its scales
         // (N is a multiple of 16, scales of 16-byte alignment: four at a time)
-        *reinterpret_cast<float4*>(my_scale + 4 * lane) =
-            n < p.N ? *reinterpret_cast<const float4*>(s + n) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 v = n < p.N ? *reinterpret_cast<const float4*>(s + n) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(my_scale + 4 * lane) = v;
+        huge = __any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) > kFirstScale);
         __syncwarp();
       }
       ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * buf, use & 1u, abort_flag, p.status));
@@ -461,22 +476,26 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           slab_add<32>(part0, (size_t)EPI_WARPS * L_PART, q.slices, q.slice, c / 4, lane, a);
           if constexpr (SWIGLU) slab_add<32>(part0, (size_t)EPI_WARPS * L_PART, q.slices, q.slice, (COLS + c) / 4, lane, u);
         }
+        auto store = [&](auto scale) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 2 * PER) {
-          uint4 v[2];
+          for (int j = 0; j < 32; j += 2 * PER) {
+            uint4 v[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float f[PER];
+            for (int h = 0; h < 2; ++h) {
+              float f[PER];
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const int x = j + h * PER + i;
-              f[i] = __int2float_rn((int)a[x]) * rs * my_scale[c + x];
-              if constexpr (SWIGLU) f[i] = swiglu<T>(f[i], __int2float_rn((int)u[x]) * rs * my_scale[64 + c + x]);
+              for (int i = 0; i < PER; ++i) {
+                const int x = j + h * PER + i;
+                f[i] = scale(a[x], my_scale[c + x], rs);
+                if constexpr (SWIGLU) f[i] = swiglu<T>(f[i], scale(u[x], my_scale[64 + c + x], rs));
+              }
+              v[h] = Out<T>::pack(f);
             }
-            v[h] = Out<T>::pack(f);
+            if (row_ok && n0 + c + j < p.N) store_sector(dst + c + j, v[0], v[1], p.sectors);       // (N is a multiple of 16)
           }
-          if (row_ok && n0 + c + j < p.N) store_sector(dst + c + j, v[0], v[1], p.sectors);       // (N is a multiple of 16)
-        }
+        };
+        if (huge) store([](uint32_t acc, float channel, float row) { return scaled_any(acc, channel, row); });
+        else      store([](uint32_t acc, float channel, float row) { return scaled(acc, channel, row); });
       }
       tc_fence_before();
       __syncwarp();
@@ -663,7 +682,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const float rs = __shfl_sync(0xffffffffu, my_rs, c);
-          const float v0 = __int2float_rn((int)a0[c]) * rs * s0, v1 = NARROW ? 0.f : __int2float_rn((int)a1[c]) * rs * s1;
+          const float v0 = scaled_any(a0[c], s0, rs), v1 = NARROW ? 0.f : scaled_any(a1[c], s1, rs);
           if (c >= n_valid) continue;
           if (SWIGLU) {
             if (n < p.N) out[(size_t)c * p.N + n] = Out<T>::one(swiglu<T>(v0, v1));

@@ -533,3 +533,36 @@ def test_more_tiles_than_22_bits_count():
         assert int(torch.count_nonzero(out[300:2 ** 28 - 200])) + int(torch.count_nonzero(out[2 ** 29 + 200:M - 300])) == 0
         del out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M", [5, 300])
+def test_scales_of_any_size(M, dtype):
+    """Infinity only where the product itself is that large: sums of 2^20 and more times a scale of 1e33 on either side, the other
+    one small.  Rows and channels of every size meet; both kernels, plain and SwiGLU."""
+    K, N, E = 4096, 320, 2
+    a, w = make_codes((M, K), 1), make_codes((E, K, N), 2)
+    a[:, :64], w[:, :64] = 127, 127                     # no sum near zero
+    a[0], w[1, :, 3] = 0, 0                             # but these are
+    offsets = torch.tensor([0, M // 2, M], dtype=torch.int32)
+    rs = torch.tensor([1.0, 1e33, 1e-4, 3e-39, 1e-33, 2e29])[torch.arange(M) % 6]
+    cs = torch.tensor([1e-4, 1e33, 1.0, 1e-33, 3e-39, 2e29])[torch.arange(E * N) % 6].view(E, N)
+    args = [t.to(DEV) for t in (a, rs, offsets, w, cs)]
+    out = bw.int8_grouped_gemm(*args, out_dtype=dtype)
+    ones = torch.full((E, N), 1e-3, device=DEV)         # gates of ordinary rows; up products of every size
+    h = bw.int8_grouped_swiglu(args[0], args[1], args[2], args[3], args[3], ones, args[4], out_dtype=dtype)
+    seen = 0
+    top = torch.finfo(dtype).max
+    for e, (lo, hi) in enumerate(((0, M // 2), (M // 2, M))):
+        acc = args[0][lo:hi].double() @ args[3][e].double()
+        ref = acc * args[1][lo:hi, None].double() * args[4][e].double()
+        fits, past = ref.abs() <= top * (1 - 2.0 ** -7), ref.abs() > top * (1 + 2.0 ** -7)
+        bound = ref.abs() * (3.01 * U32 + half_step(dtype) * 1.001) + smallest_step(dtype)
+        seen += int(past.sum())
+        assert ((out[lo:hi].double() - ref).abs() <= bound)[fits].all(), e
+        assert (out[lo:hi].isinf() & (out[lo:hi].double().sign() == ref.sign()))[past].all(), e
+        gate = acc * args[1][lo:hi, None].double() * ones[0, 0].double()
+        want, bound = swiglu_bound(gate, ref, dtype)
+        live = fits & (want.abs() <= top * (1 - 2.0 ** -7)) & (gate.abs() < 1e3)
+        assert live.any() and ((h[lo:hi].double() - want).abs() <= bound)[live].all(), e
+    assert seen
