@@ -260,10 +260,20 @@ __device__ __forceinline__ float scaled_any(uint32_t acc, float channel, float r
   return scaled(acc, row_first ? row : channel, row_first ? channel : row);
 }
 
-// fp32 results get the accurate exponential and division, 16-bit ones the fast forms (2^-21 against a rounding of 2^-9)
+// silu(g) * u with the accurate exponential and a quotient that is rounded like a division's.  16-bit results get the quotient
+// from the reciprocal and one Newton step on what is left over (Markstein's correction), which needs no branch per element: half
+// a step and 2^-22 of one.  (What is left over is NaN where g or d is infinite; then the first estimate is the result.  From
+// d = 2^126 on the reciprocal is 0, and so is the result instead of a number below 2^-119.)  With __expf and __fdividef, whose
+// error of 2 + 1.16 |g| steps grows with the gate, one 16-bit result in 4000 was rounded the other way, and where it was a row's
+// largest, every code of the row followed.  Cost at 64 experts of 2048 x 1408, 768 rows each: 212 -> 218 us (222 with the
+// division); 384 rows 126 -> 128, decode batches and fp32 results nothing.
 template <class T> __device__ __forceinline__ float swiglu(float g, float u) {
-  if constexpr (sizeof(T) == 4) return g / (1.0f + expf(-g)) * u;
-  else                          return silu_f(g) * u;
+  const float d = 1.0f + expf(-g);
+  if constexpr (sizeof(T) == 4) return g / d * u;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  const float q = g * r, rest = fmaf(-d, q, g);
+  return (rest == rest ? fmaf(rest, r, q) : q) * u;
 }
 
 // Rows in front of the first segment and behind the last belong to no expert: zeros.  `part` of `parts` threads.
