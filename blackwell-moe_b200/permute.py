@@ -4,7 +4,7 @@ The permutation of the MoE block as operators of their own, for programs that ru
 - experts in another format, an adapter, a training step: ``permute_tokens`` takes over ``permute_tokens``
 (src/blackwell_moe/kernels/permute.py:12-39), ``unpermute_tokens`` takes over ``unpermute_and_combine``
 (src/blackwell_moe/kernels/permute.py:42-59).  bf16, fp16 and fp32; sums are held in fp32, added in a fixed order and
-rounded once.  Both are differentiable (once): in the tokens and the rows, and in the routing weights.
+rounded once.  Both are differentiable (once, forwards or backwards): in the tokens and the rows, and in the routing weights.
 """
 
 from __future__ import annotations
@@ -13,6 +13,7 @@ import functools
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .moe import _contig, _on_device, _require_cuda, _stream
@@ -168,33 +169,51 @@ def _unpermute_backward(dout, rows, offsets, pos, weights, rows_grad, weights_gr
     return drows, dweights
 
 
+def _has_tangent(*tensors):
+    """Whether one of them is a dual tensor, for which ``requires_grad`` need not be set: the launches know nothing of tangents."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _once(backward):
     """``once_differentiable`` where a second derivative could be asked for (``create_graph``): its bookkeeping costs as
     much as a small batch's backward pass."""
     guarded = torch.autograd.function.once_differentiable(backward)
-    return staticmethod(lambda ctx, grad: guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad))
+
+    def call(ctx, grad):
+        if forward_ad._current_level >= 0 and _has_tangent(grad, *ctx.saved_tensors):
+            raise NotImplementedError("the gradients of permute_tokens and unpermute_tokens have no derivative themselves")
+        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+    return staticmethod(call)
 
 
 def _permute_backward(ctx, drows):
     return _unpermute(drows.contiguous(), ctx.saved_tensors[0], None), None, None
 
 
+def _permute_jvp(ctx, dx, *_):
+    return _permute(dx.contiguous(), *ctx.saved_tensors)
+
+
 class _PermuteRows(torch.autograd.Function):
-    backward = _once(_permute_backward)
+    backward, jvp = _once(_permute_backward), staticmethod(_permute_jvp)
 
     @staticmethod
     def forward(ctx, x, offsets, pos):
         ctx.save_for_backward(pos)
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(offsets, pos)
         return _permute(x, offsets, pos)
 
 
 class _PermuteTokens(torch.autograd.Function):
-    backward = _once(_permute_backward)
+    backward, jvp = _once(_permute_backward), staticmethod(_permute_jvp)
 
     @staticmethod
     def forward(ctx, x, args, found):        # args: (indices, num_experts); the plan leaves through the list `found`
         rows, plan = _permute_new(x, *args)
         ctx.save_for_backward(plan.pos)
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(plan.offsets, plan.pos)
         found.append(plan)
         return rows
 
@@ -208,13 +227,24 @@ def _unpermute_rows_backward(ctx, dout):
     return drows, None, None, dweights
 
 
+def _unpermute_rows_jvp(ctx, drows, _offsets, _pos, dweights):
+    rows, pos, weights = ctx.saved_tensors
+    # (a sum of two results that are rounded to the type each)
+    terms = [] if drows is None else [_unpermute(drows.contiguous(), pos, weights)]
+    if dweights is not None:
+        terms.append(_unpermute(rows, pos, dweights.contiguous()))
+    return sum(terms[1:], start=terms[0])
+
+
 class _UnpermuteRows(torch.autograd.Function):
-    backward = _once(_unpermute_rows_backward)
+    backward, jvp = _once(_unpermute_rows_backward), staticmethod(_unpermute_rows_jvp)
 
     @staticmethod
     def forward(ctx, rows, offsets, pos, weights):
-        # the rows are kept for the weights' gradient only
+        # the rows are kept for the weights' derivative only
         ctx.save_for_backward(rows if ctx.needs_input_grad[3] else None, offsets, pos, weights)
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(rows, pos, weights)
         return _unpermute(rows, pos, weights)
 
 
@@ -227,7 +257,7 @@ def permute_tokens(x: torch.Tensor, indices: torch.Tensor = None, num_experts: i
     _contig(x, "x")
     if (indices is None) == (plan is None) or (indices is None) != (num_experts is None):
         raise ValueError("permute_tokens takes indices and num_experts, or a plan")
-    wants_grad = x.requires_grad and torch.is_grad_enabled()
+    wants_grad = (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x)
     if plan is None:
         _check_indices(indices, num_experts)
         assert indices.shape[0] == x.shape[0], (indices.shape, x.shape)
@@ -262,7 +292,8 @@ def unpermute_tokens(rows: torch.Tensor, plan: PermutePlan, weights: torch.Tenso
     """``rows[T*K,D]`` in expert order -> ``out[T,D]``, ``out[t] = sum_k weights[t,k] * rows[plan.pos[t,k]]`` with
     ``weights[T,K]`` fp32 (absent: 1).  Slots without a row add nothing.  Differentiable in ``rows`` and ``weights``."""
     offsets, pos = _check_unpermute(rows, plan, weights)
-    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+    if (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))) \
+            or _has_tangent(rows, weights):
         return _UnpermuteRows.apply(rows, offsets, pos, weights)
     return _unpermute(rows, pos, weights)
 

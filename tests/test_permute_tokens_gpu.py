@@ -305,3 +305,48 @@ def test_places_outside_the_rows_are_no_rows():
     assert torch.equal(out, rows[[0, 3, 1, 2]])
     back, _ = bw.permute_tokens(out, plan=plan)
     assert torch.equal(back[:4], rows[:4])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_forward_mode_derivatives(dtype):
+    """Dual tensors, which need not require a gradient.  Whole numbers: every sum is exact, and so is the derivative."""
+    from torch.autograd import forward_ad as fw
+    T, D, E, K = 19, 40, 8, 3
+    idx, _ = routing(T, E, K, 3, bad=2)
+    idx = idx.to(DEV)
+    g = torch.Generator().manual_seed(5)
+    whole = lambda *shape: torch.randint(-2, 3, shape, generator=g).float().to(DEV)                     # noqa: E731
+    x, dx, r, dr = (whole(*s).to(dtype) for s in ((T, D), (T, D), (T * K, D), (T * K, D)))
+    w, dw = whole(T, K), whole(T, K)
+    want, plan = bw.permute_tokens(dx, idx, E)
+    for grad in (False, True):
+        with fw.dual_level():
+            dual = fw.make_dual(x.clone().requires_grad_(grad), dx)
+            for rows in (bw.permute_tokens(dual, idx, E)[0], bw.permute_tokens(dual, plan=plan)[0]):
+                assert torch.equal(fw.unpack_dual(rows).tangent, want)
+                assert torch.equal(rows.detach(), bw.permute_tokens(x, plan=plan)[0])
+            rd, wd = fw.make_dual(r.clone().requires_grad_(grad), dr), fw.make_dual(w.clone().requires_grad_(grad), dw)
+            tangent = lambda *a: fw.unpack_dual(bw.unpermute_tokens(*a)).tangent                        # noqa: E731
+            assert torch.equal(tangent(rd, plan), bw.unpermute_tokens(dr, plan))
+            assert torch.equal(tangent(rd, plan, w), bw.unpermute_tokens(dr, plan, w))
+            assert torch.equal(tangent(r, plan, wd), bw.unpermute_tokens(r, plan, dw))
+            assert torch.equal(tangent(rd, plan, wd), bw.unpermute_tokens(dr, plan, w) + bw.unpermute_tokens(r, plan, dw))
+            # a tensor that is no dual inside the level
+            assert fw.unpack_dual(bw.unpermute_tokens(r, plan, w)).tangent is None
+    assert torch.equal(bw.unpermute_tokens(r, plan, w), bw.unpermute_tokens(r.clone(), plan, w.clone()))
+
+
+def test_no_derivative_of_a_gradient():
+    """Forward over reverse: the gradients are not differentiable themselves, and say so."""
+    from torch.autograd import forward_ad as fw
+    idx, w = routing(6, 4, 2, 0)
+    x, v = torch.randn(6, 40, device=DEV), torch.randn(6, 40, device=DEV)
+    with fw.dual_level():
+        leaf = x.clone().requires_grad_()
+        rows, plan = bw.permute_tokens(fw.make_dual(leaf, v), idx.to(DEV), 4)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(rows.square().sum(), leaf)
+        r, wt = torch.randn(12, 40, device=DEV, requires_grad=True), fw.make_dual(w.to(DEV), torch.ones(6, 2, device=DEV))
+        out = bw.unpermute_tokens(r, plan, wt)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(out.sum(), r)
