@@ -73,7 +73,7 @@ inline cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+inline int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }      // (a + b may leave 32 bits)
 inline size_t dtype_bytes(int dtype) { return dtype == BWMOE_F32 ? 4 : 2; }
 template <class T> struct TypeTag { using type = T; };
 // Rows at most, where sizes that round up to a tile stay in 32 bits (permutation, 8-bit integers).

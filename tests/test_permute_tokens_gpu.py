@@ -350,3 +350,28 @@ def test_no_derivative_of_a_gradient():
         out = bw.unpermute_tokens(r, plan, wt)
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(out.sum(), r)
+
+
+def test_the_largest_number_of_rows():
+    """As many slots as are accepted: the plan's blocks have 2^23 slots each, which takes the sum in a rounded-up quotient past
+    32 bits."""
+    T, E = 2 ** 31 - 4096, 3
+    idx = torch.zeros(T, 1, dtype=torch.int32, device=DEV)
+    idx[-5000:] = 1
+    idx[5], idx[2 ** 30], idx[T - 3] = 2, -1, 2
+    x = torch.zeros(T, 1, dtype=BF16, device=DEV)
+    for i, t in enumerate((0, 5, 6, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 1, T - 5001, T - 5000, T - 3, T - 1)):
+        x[t] = i + 1
+    rows, plan = bw.permute_tokens(x, idx, E)
+    zeros, ones = T - 5000 - 2, 4999
+    assert plan.offsets.tolist() == [0, zeros, zeros + ones, T - 1]
+    places = {0: 0, 5: T - 3, 6: 5, 2 ** 30 - 1: 2 ** 30 - 2, 2 ** 30: -1, 2 ** 30 + 1: 2 ** 30 - 1, T - 5001: zeros - 1,
+              T - 5000: zeros, T - 3: T - 2, T - 1: zeros + ones - 1}
+    for t, p in places.items():
+        assert int(plan.pos[t, 0]) == p, t
+        if p >= 0:
+            assert int(plan.row_slot[p]) == t and float(rows[p]) == float(x[t]), t
+    assert int(plan.row_slot[T - 1]) == -1 and float(rows[T - 1]) == 0 and int(torch.count_nonzero(rows)) == 9
+    assert torch.equal(bw.unpermute_tokens(rows, plan)[:7], x[:7])
+    del idx, x, rows, plan
+    torch.cuda.empty_cache()
