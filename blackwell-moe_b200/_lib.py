@@ -81,6 +81,7 @@ SIGNATURES = {
     "bwmoe_scatter_quant_peers": (_i, [_vp, _ip, _ip, _fp, _ip, _i, _i, _i, _i, C.POINTER(C.c_void_p), _i, _i, _ip,
                                        _vp]),
     "bwmoe_permute_tokens": (_i, [_vp, _ip] + [_i] * 5 + [_ip] * 4 + [_vp, _ip, _vp, _vp]),
+    "bwmoe_plan_row_slots": (_i, [_ip, _i, _i, _ip, _vp]),
     "bwmoe_permute_rows": (_i, [_vp, _ip, _ip] + [_i] * 5 + [_vp, _vp]),
     "bwmoe_unpermute_rows": (_i, [_vp, _ip, _fp] + [_i] * 4 + [_vp, _vp]),
     "bwmoe_unpermute_rows_backward": (_i, [_vp, _vp, _ip, _ip, _fp] + [_i] * 5 + [_vp, _fp, _vp]),

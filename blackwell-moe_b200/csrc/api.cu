@@ -893,6 +893,10 @@ int bwmoe_permute_tokens(const void* x, const int32_t* indices, int T, int D, in
   return launch_permute_rows(x, pos, offsets, T, D, E, K, dtype, rows, st);
 }
 
+int bwmoe_plan_row_slots(const int32_t* pos, int T, int K, int32_t* row_slot, void* stream) {
+  return launch_row_slots(pos, T, K, row_slot, static_cast<cudaStream_t>(stream));
+}
+
 int bwmoe_permute_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype, void* rows,
                        void* stream) {
   return launch_permute_rows(x, pos, offsets, T, D, E, K, dtype, rows, static_cast<cudaStream_t>(stream));

@@ -292,7 +292,8 @@ int launch_scatter_rows_group_peers(const void* xq_tok, const float* inv_tok, co
 bool plan_permute_applicable(int T, int E, int K);
 int launch_plan_permute(const void* x, const int32_t* indices, int T, int E, int K, size_t row_bytes, int32_t* offsets, int32_t* pos,
                         int32_t* row_slot, int32_t* row_expert, int32_t* status, void* rows, cudaStream_t st);
-// Tokens into expert order and back (permute_rows.cu)
+// Tokens into expert order and back (permute_rows.cu).  E = 0: the plan is not this library's, and `offsets` are its rows' slots.
+int launch_row_slots(const int32_t* pos, int T, int K, int32_t* row_slot, cudaStream_t st);
 int launch_permute_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
                         void* rows, cudaStream_t st);
 int launch_unpermute_rows(const void* rows, const int32_t* pos, const float* weights, int T, int D, int K, int dtype, void* out,

@@ -1,6 +1,8 @@
 // Tokens into expert order and back, with gradients.  M = T * K rows; pos[t,k] is the row of slot (t,k), -1 where the
-// slot's expert id was out of range, and the rows offsets[E] .. M-1 then belong to no slot.
+// slot's expert id was out of range, and the rows offsets[E] .. M-1 then belong to no slot.  (A plan made elsewhere may leave out
+// any row.)
 //
+//   row slots          slots[pos[t,k]] = (t,k), else -1                  for plans made elsewhere (no_slot() reads it)
 //   permute            rows[pos[t,k]] = x[t]                             its gradient:  dx[t] = sum_k drows[pos[t,k]]
 //   unpermute          out[t] = sum_k w[t,k] * rows[pos[t,k]]            (w absent: 1)
 //   unpermute backward drows[pos[t,k]] = w[t,k] * dout[t]                dw[t,k] = < rows[pos[t,k]], dout[t] >
@@ -42,6 +44,15 @@ __device__ __forceinline__ int row_of(const int32_t* __restrict__ pos, long long
   return (unsigned)p < (unsigned)M ? p : -1;
 }
 
+__global__ void __launch_bounds__(kThreads)
+row_slots_kernel(const int32_t* __restrict__ pos, int M, int32_t* __restrict__ slots) {
+  chain_wait();
+  const long long s = (long long)blockIdx.x * kThreads + threadIdx.x;
+  if (s >= M) return;
+  const int p = row_of(pos, s, M);
+  if (p >= 0) slots[p] = (int)s;
+}
+
 // `lanes` threads (a power of two) stand side by side on one token's row, each with U pieces.
 template <int BYTES>
 __global__ void __launch_bounds__(kThreads)
@@ -57,16 +68,17 @@ permute_rows_kernel(const typename Piece<BYTES>::type* __restrict__ x, const int
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (c0 + u * lanes < pieces) v[u] = x[(size_t)t * pieces + c0 + u * lanes];
-  const int M = T * K, n_rows = offsets[E];
+  const int M = T * K, n_rows = E > 0 ? offsets[E] : 0;
 #pragma unroll 4
   for (int k = 0; k < K; ++k) {
     const int s = t * K + k, p = row_of(pos, s, M);
+    const bool none = no_slot(offsets, E, n_rows, s);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int c = c0 + u * lanes;
       if (c >= pieces) continue;
       if (p >= 0) rows[(size_t)p * pieces + c] = v[u];
-      if (s >= n_rows) rows[(size_t)s * pieces + c] = zero_piece<P>();
+      if (none) rows[(size_t)s * pieces + c] = zero_piece<P>();
     }
   }
 }
@@ -147,16 +159,18 @@ unpermute_rows_backward_kernel(const typename Piece<BYTES>::type* __restrict__ d
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = blockIdx.x * (kThreads / 32 / wpt) + warp / wpt, sub = warp % wpt;
   const bool live = t < n_tok;
-  const int M = n_tok * K, n_rows = DROWS ? offsets[E] : M;
+  const int M = n_tok * K, n_rows = DROWS && E > 0 ? offsets[E] : 0;
   for (int k0 = 0; k0 < K; k0 += R) {
     int p[R];
     float w[R], dot[R];
+    unsigned none = 0;                              // rows (of the slots' numbers) that no slot owns
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       const bool slot = live && k0 + j < K;
       p[j] = slot ? row_of(pos, (size_t)t * K + k0 + j, M) : -1;
       w[j] = DROWS && slot ? weights[(size_t)t * K + k0 + j] : 0.f;
       dot[j] = 0.f;
+      if (DROWS && slot && no_slot(offsets, E, n_rows, t * K + k0 + j)) none |= 1u << j;
     }
     for (int c = sub * 32 + lane; live && c < pieces; c += 32 * wpt) {
       Values<T, BYTES> d, q[R];
@@ -168,7 +182,7 @@ unpermute_rows_backward_kernel(const typename Piece<BYTES>::type* __restrict__ d
       }
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        if (DROWS && k0 + j < K && t * K + k0 + j >= n_rows) drows[(size_t)(t * K + k0 + j) * pieces + c] = zero_piece<P>();
+        if (DROWS && (none >> j & 1u)) drows[(size_t)(t * K + k0 + j) * pieces + c] = zero_piece<P>();
         if (p[j] < 0) continue;
         if constexpr (DW) {
 #pragma unroll
@@ -306,10 +320,18 @@ int for_type_and_piece(int dtype, int bytes, F fn) {
 
 }  // namespace
 
+int launch_row_slots(const int32_t* pos, int T, int K, int32_t* row_slot, cudaStream_t st) {
+  if (int rc = check_rows("plan_row_slots", T, 1, K, BWMOE_F32)) return rc;
+  BWMOE_REQUIRE(pos && row_slot, BWMOE_ERR_NULL, "plan_row_slots: null pointer");
+  BWMOE_CUDA_OK(cudaMemsetAsync(row_slot, 0xff, sizeof(int32_t) * (size_t)T * K, st));
+  BWMOE_CUDA_OK(launch_chained(row_slots_kernel, dim3((unsigned)ceil_div(T * K, kThreads)), dim3(kThreads), 0, st, pos, T * K, row_slot));
+  return BWMOE_OK;
+}
+
 int launch_permute_rows(const void* x, const int32_t* pos, const int32_t* offsets, int T, int D, int E, int K, int dtype,
                         void* rows, cudaStream_t st) {
   if (int rc = check_rows("permute_rows", T, D, K, dtype)) return rc;
-  BWMOE_REQUIRE(E > 0, BWMOE_ERR_BAD_SHAPE, "permute_rows: E=%d", E);
+  BWMOE_REQUIRE(E >= 0, BWMOE_ERR_BAD_SHAPE, "permute_rows: E=%d", E);
   BWMOE_REQUIRE(x && pos && offsets && rows, BWMOE_ERR_NULL, "permute_rows: null pointer");
   if (int rc = check_align("permute_rows", dtype, {x, rows})) return rc;
   const size_t row_bytes = (size_t)D * dtype_bytes(dtype);
@@ -337,7 +359,7 @@ int launch_unpermute_rows_backward(const void* dout, const void* rows, const int
                                    cudaStream_t st) {
   if (int rc = check_rows("unpermute_rows_backward", T, D, K, dtype)) return rc;
   BWMOE_REQUIRE(dout && pos && (drows || dweights), BWMOE_ERR_NULL, "unpermute_rows_backward: null pointer");
-  BWMOE_REQUIRE(!drows || (offsets && weights && E > 0), BWMOE_ERR_NULL,
+  BWMOE_REQUIRE(!drows || (offsets && weights && E >= 0), BWMOE_ERR_NULL,
                 "unpermute_rows_backward: the rows' gradient needs offsets and weights");
   BWMOE_REQUIRE(!dweights || rows, BWMOE_ERR_NULL, "unpermute_rows_backward: the weights' gradient needs the rows");
   if (int rc = check_align("unpermute_rows_backward", dtype, {dout, rows, drows})) return rc;

@@ -19,6 +19,12 @@ template <class P> __device__ __forceinline__ P zero_piece() {
   return z;
 }
 
+// Whether no slot owns row r.  E > 0: the plan is this library's, `offsets` are its segments [E + 1], and the rows without a slot
+// are those behind the last (n_rows = offsets[E]).  E = 0: any plan, and `offsets` is a slot of each row, -1 where there is none.
+__device__ __forceinline__ bool no_slot(const int32_t* __restrict__ offsets, int E, int n_rows, int r) {
+  return E > 0 ? r >= n_rows : offsets[r] < 0;
+}
+
 // Bytes of the widest piece that divides the row and every pointer.
 inline int piece_bytes(size_t row_bytes, std::initializer_list<const void*> ptrs) {
   uintptr_t bits = (uintptr_t)row_bytes;

@@ -18,7 +18,7 @@
 // the codes - and written to all of the rows it is needed in (the K rows of its token, or one).  The conversion adds
 // 1.5 * 2^23 instead of converting (the low byte of the sum is the code): at 3 bytes per element the conversion unit
 // (16 results per cycle and SM) would be as busy as the memory.
-#include "common.cuh"
+#include "pieces.cuh"
 
 namespace bwmoe {
 namespace {
@@ -197,7 +197,7 @@ quant_int8_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ pos,
   }
   if (!live) return;
   const RowScale r = row_scale<T>(m);
-  const int M = n_tok * K, n_rows = pos != nullptr ? offsets[E] : M;
+  const int M = n_tok * K, n_rows = pos != nullptr && E > 0 ? offsets[E] : 0;
   auto store = [&](int c, uint4 o) {
     if (pos == nullptr) {
       reinterpret_cast<uint4*>(codes + (size_t)t * D)[c] = o;
@@ -211,7 +211,7 @@ quant_int8_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ pos,
         reinterpret_cast<uint4*>(codes + (size_t)p * D)[c] = o;
         if (c == 0) scales[p] = r.scale;
       }
-      if (s >= n_rows) {                        // a row that no slot owns
+      if (no_slot(offsets, E, n_rows, s)) {
         reinterpret_cast<uint4*>(codes + (size_t)s * D)[c] = make_uint4(0u, 0u, 0u, 0u);
         if (c == 0) scales[s] = 0.f;
       }
@@ -235,7 +235,7 @@ int launch_quant_int8_rows(const void* x, const int32_t* pos, const int32_t* off
   BWMOE_REQUIRE((long long)T * K <= kMaxRows, BWMOE_ERR_UNSUPPORTED, "int_quant: T*K too large");
   BWMOE_REQUIRE(dtype >= BWMOE_BF16 && dtype <= BWMOE_F32, BWMOE_ERR_UNSUPPORTED, "int_quant: unknown type %d", dtype);
   BWMOE_REQUIRE(x && codes && scales, BWMOE_ERR_NULL, "int_quant: null pointer");
-  BWMOE_REQUIRE(pos == nullptr ? K == 1 : (offsets != nullptr && E > 0), BWMOE_ERR_BAD_SHAPE,
+  BWMOE_REQUIRE(pos == nullptr ? K == 1 : (offsets != nullptr && E >= 0), BWMOE_ERR_BAD_SHAPE,
                 "int_quant: K=%d needs the slots' places and the segments' offsets", K);
   BWMOE_REQUIRE(aligned16(x) && aligned16(codes) && reinterpret_cast<uintptr_t>(scales) % 4 == 0, BWMOE_ERR_BAD_ALIGN,
                 "int_quant: x and codes must be 16-byte aligned");

@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from .moe import _contig, _on_device, _require_cuda, _stream, _thread_workspace
-from .permute import _DTYPES, _MAX_SIZE, _check_plan, _check_sizes, _dtype_code
+from .permute import _DTYPES, _MAX_SIZE, _check_plan, _check_sizes, _dtype_code, _is_own, _row_owners
 
 _I8 = torch.int8
 
@@ -40,19 +40,20 @@ def quantize_tokens_int8(x: torch.Tensor, plan=None):
     T, D = x.shape
     if D == 0 or D % 16:
         raise ValueError(f"D={D} must be a multiple of 16")
-    tensors, K, E = [_contig(x, "x")], 1, 1
+    tensors, K = [_contig(x, "x")], 1
     if plan is not None:
         offsets, pos = _check_plan(plan)
         assert pos.shape[0] == T, (pos.shape, x.shape)
         tensors += [offsets, pos]
-        K, E = pos.shape[1], offsets.numel() - 1
+        K = pos.shape[1]
     dev = _require_cuda(*tensors)
     codes = torch.empty((T * K, D), dtype=_I8, device=dev)
     scales = torch.empty(T * K, dtype=torch.float32, device=dev)
     if T:
         with _on_device(dev):
+            owners, E = _row_owners(offsets, pos, _is_own(plan)) if plan is not None else (None, 1)
             _lib.check(_lib.lib().bwmoe_int_quant(x.data_ptr(), pos.data_ptr() if plan is not None else None,
-                                                  offsets.data_ptr() if plan is not None else None, T, D, E, K, code,
+                                                  owners.data_ptr() if plan is not None else None, T, D, E, K, code,
                                                   codes.data_ptr(), scales.data_ptr(), _stream(dev)))
     return codes, scales
 

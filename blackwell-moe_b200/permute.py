@@ -27,11 +27,35 @@ class PermutePlan(NamedTuple):
     ``offsets[E+1]``: expert e's rows are ``offsets[e] .. offsets[e+1]-1``; ``pos[T,K]``: the row of each slot;
     ``row_slot[M]``: the slot of each row, ``t*K + k``; ``row_expert[M]``: its expert.  A slot whose expert id is
     outside ``[0, E)`` has no row (``pos`` -1), and the rows past ``offsets[E]`` then have no slot (-1).  The operators
-    read ``offsets`` and ``pos`` only: a plan made elsewhere may leave the other two out."""
+    read ``offsets`` and ``pos`` only: a plan made elsewhere, or one with slots dropped (``pos`` set to -1), may leave the
+    other two out, and may leave any row without a slot.  Two slots never have the same row."""
     offsets: torch.Tensor
     pos: torch.Tensor
     row_slot: Optional[torch.Tensor] = None
     row_expert: Optional[torch.Tensor] = None
+
+
+class _OwnPlan(PermutePlan):
+    """A plan as the library wrote it: the rows without a slot are those past ``offsets[E]``."""
+    __slots__ = ()
+    _make = PermutePlan._make           # what _replace() returns is not
+
+
+def _is_own(plan) -> bool:
+    if type(plan) is not _OwnPlan:
+        return False
+    offsets, pos = plan[0], plan[1]
+    return not (pos.is_inference() or offsets.is_inference()) and pos._version == 0 and offsets._version == 0
+
+
+def _row_owners(offsets, pos, own):
+    """What tells the rows without a slot: the segments of the library's own plan, or each row's slot.  The tensor, and its
+    number of experts (0)."""
+    if own:
+        return offsets, offsets.numel() - 1
+    slots = pos.new_empty(pos.numel())
+    _lib.check(_lib.lib().bwmoe_plan_row_slots(pos.data_ptr(), *pos.shape, slots.data_ptr(), _stream(pos.device)))
+    return slots, 0
 
 
 _MAX_SIZE = 2 ** 31 - 4096      # sizes reach the library as 32-bit integers: a larger one would wrap on the way
@@ -62,7 +86,7 @@ def _empty_plan(indices, T, K, num_experts, scratch_bytes):
     # (not views of one another: each has its own version, as tensors that were allocated apart)
     o, p, s, e, rest = torch.unsafe_split_with_sizes(indices.new_empty(num_experts + 1 + 3 * M + extra), (num_experts + 1, M, M, M, extra))
     status = rest.data_ptr()
-    return PermutePlan(o, p.view(T, K), s, e), status, status + 16
+    return _OwnPlan(o, p.view(T, K), s, e), status, status + 16
 
 
 def _check_indices(indices, num_experts):
@@ -124,16 +148,17 @@ def _permute_new(x, indices, num_experts):
     return rows, plan
 
 
-def _permute(x, offsets, pos):
+def _permute(x, offsets, pos, own):
     """rows[pos[t,k]] = x[t]"""
     dev = x.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
-            return _permute(x, offsets, pos)
+            return _permute(x, offsets, pos, own)
     (T, K), D = pos.shape, x.shape[1]
     rows = x.new_empty((T * K, D))
     if T and D:
-        _lib.check(_lib.lib().bwmoe_permute_rows(x.data_ptr(), pos.data_ptr(), offsets.data_ptr(), T, D, offsets.numel() - 1,
+        owners, E = _row_owners(offsets, pos, own)
+        _lib.check(_lib.lib().bwmoe_permute_rows(x.data_ptr(), pos.data_ptr(), owners.data_ptr(), T, D, E,
                                                  K, _DTYPES[x.dtype], rows.data_ptr(), _stream(dev)))
     return rows
 
@@ -152,7 +177,7 @@ def _unpermute(rows, pos, weights):
     return out
 
 
-def _unpermute_backward(dout, rows, offsets, pos, weights, rows_grad, weights_grad):
+def _unpermute_backward(dout, rows, offsets, pos, own, weights, rows_grad, weights_grad):
     T, K = pos.shape
     D, dev = dout.shape[1], dout.device
     with _on_device(dev):
@@ -160,9 +185,10 @@ def _unpermute_backward(dout, rows, offsets, pos, weights, rows_grad, weights_gr
         dweights = torch.empty_like(weights) if weights_grad else None
         if T and D:
             if rows_grad or weights_grad:
+                owners, E = _row_owners(offsets, pos, own or not rows_grad)
                 _lib.check(_lib.lib().bwmoe_unpermute_rows_backward(
-                    dout.data_ptr(), rows.data_ptr() if weights_grad else None, pos.data_ptr(), offsets.data_ptr(),
-                    weights.data_ptr(), T, D, offsets.numel() - 1, K, _DTYPES[dout.dtype], drows.data_ptr() if rows_grad else None,
+                    dout.data_ptr(), rows.data_ptr() if weights_grad else None, pos.data_ptr(), owners.data_ptr(),
+                    weights.data_ptr(), T, D, E, K, _DTYPES[dout.dtype], drows.data_ptr() if rows_grad else None,
                     dweights.data_ptr() if weights_grad else None, _stream(dev)))
         elif weights_grad:
             dweights.zero_()
@@ -187,22 +213,23 @@ def _once(backward):
 
 
 def _permute_backward(ctx, drows):
-    return _unpermute(drows.contiguous(), ctx.saved_tensors[0], None), None, None
+    return _unpermute(drows.contiguous(), ctx.saved_tensors[0], None), None, None, None
 
 
 def _permute_jvp(ctx, dx, *_):
-    return _permute(dx.contiguous(), *ctx.saved_tensors)
+    return _permute(dx.contiguous(), *ctx.saved_tensors, ctx.own)
 
 
 class _PermuteRows(torch.autograd.Function):
     backward, jvp = _once(_permute_backward), staticmethod(_permute_jvp)
 
     @staticmethod
-    def forward(ctx, x, offsets, pos):
+    def forward(ctx, x, offsets, pos, own):
         ctx.save_for_backward(pos)
         if forward_ad._current_level >= 0:
             ctx.save_for_forward(offsets, pos)
-        return _permute(x, offsets, pos)
+            ctx.own = own
+        return _permute(x, offsets, pos, own)
 
 
 class _PermuteTokens(torch.autograd.Function):
@@ -214,6 +241,7 @@ class _PermuteTokens(torch.autograd.Function):
         ctx.save_for_backward(plan.pos)
         if forward_ad._current_level >= 0:
             ctx.save_for_forward(plan.offsets, plan.pos)
+            ctx.own = True
         found.append(plan)
         return rows
 
@@ -222,12 +250,12 @@ def _unpermute_rows_backward(ctx, dout):
     rows, offsets, pos, weights = ctx.saved_tensors
     dout = dout.contiguous()
     if weights is None:
-        return _permute(dout, offsets, pos), None, None, None
-    drows, dweights = _unpermute_backward(dout, rows, offsets, pos, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[3])
-    return drows, None, None, dweights
+        return _permute(dout, offsets, pos, ctx.own), None, None, None, None
+    drows, dweights = _unpermute_backward(dout, rows, offsets, pos, ctx.own, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[3])
+    return drows, None, None, dweights, None
 
 
-def _unpermute_rows_jvp(ctx, drows, _offsets, _pos, dweights):
+def _unpermute_rows_jvp(ctx, drows, _offsets, _pos, dweights, _own):
     rows, pos, weights = ctx.saved_tensors
     # (a sum of two results that are rounded to the type each)
     terms = [] if drows is None else [_unpermute(drows.contiguous(), pos, weights)]
@@ -240,11 +268,12 @@ class _UnpermuteRows(torch.autograd.Function):
     backward, jvp = _once(_unpermute_rows_backward), staticmethod(_unpermute_rows_jvp)
 
     @staticmethod
-    def forward(ctx, rows, offsets, pos, weights):
+    def forward(ctx, rows, offsets, pos, weights, own):
         # the rows are kept for the weights' derivative only
         ctx.save_for_backward(rows if ctx.needs_input_grad[3] else None, offsets, pos, weights)
         if forward_ad._current_level >= 0:
             ctx.save_for_forward(rows, pos, weights)
+        ctx.own = own
         return _unpermute(rows, pos, weights)
 
 
@@ -271,7 +300,8 @@ def permute_tokens(x: torch.Tensor, indices: torch.Tensor = None, num_experts: i
     offsets, pos = _check_plan(plan)
     assert pos.shape[0] == x.shape[0], (pos.shape, x.shape)
     _require_cuda(x, offsets, pos)
-    return (_PermuteRows.apply(x, offsets, pos) if wants_grad else _permute(x, offsets, pos)), plan
+    own = _is_own(plan)
+    return (_PermuteRows.apply(x, offsets, pos, own) if wants_grad else _permute(x, offsets, pos, own)), plan
 
 
 def _check_unpermute(rows, plan, weights):
@@ -294,7 +324,7 @@ def unpermute_tokens(rows: torch.Tensor, plan: PermutePlan, weights: torch.Tenso
     offsets, pos = _check_unpermute(rows, plan, weights)
     if (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))) \
             or _has_tangent(rows, weights):
-        return _UnpermuteRows.apply(rows, offsets, pos, weights)
+        return _UnpermuteRows.apply(rows, offsets, pos, weights, _is_own(plan))
     return _unpermute(rows, pos, weights)
 
 
@@ -313,4 +343,4 @@ def unpermute_tokens_backward(dout: torch.Tensor, rows: torch.Tensor, plan: Perm
         assert rows is not None and rows.shape == (T * K, D) and rows.dtype == dout.dtype, (None if rows is None else rows.shape)
         tensors.append(_contig(rows, "rows"))
     _require_cuda(*tensors)
-    return _unpermute_backward(dout, rows, offsets, pos, weights, rows_grad, weights_grad)
+    return _unpermute_backward(dout, rows, offsets, pos, _is_own(plan), weights, rows_grad, weights_grad)

@@ -503,6 +503,10 @@ int bwmoe_combine_peers(void* const* h_y_of_rank, int n_ranks, const int32_t* d_
  * results are the same on every call.  Any D; K <= 32.  Pointers are aligned to their type (rows of a multiple of 16 bytes
  * at 16-byte aligned addresses move fastest).  A place outside [0, M) is no row: its slot adds nothing, and its weight's gradient is
  * 0.  The rows d_offsets[E] .. M-1, which no slot owns (expert ids out of range), are written as zeros.
+ * That covers every row without a slot of a plan that bwmoe_permute_plan or bwmoe_permute_tokens made.  With any other plan (made
+ * elsewhere, or slots dropped from d_pos afterwards) pass E = 0 and, in the place of d_offsets, the d_row_slot that
+ * bwmoe_plan_row_slots writes for d_pos: every row that no place names is then written as zeros.  Two slots must not have the
+ * same row.
  *
  * bwmoe_permute_tokens: bwmoe_permute_plan, then bwmoe_permute_rows.  Scratch: bwmoe_plan_scratch_bytes(T, E, K).
  * replaces: permute_tokens, src/blackwell_moe/kernels/permute.py:12-39.
@@ -510,6 +514,9 @@ int bwmoe_combine_peers(void* const* h_y_of_rank, int n_ranks, const int32_t* d_
 int bwmoe_permute_tokens(const void* d_x, const int32_t* d_indices, int T, int D, int E, int K, int dtype,
                          int32_t* d_offsets, int32_t* d_pos, int32_t* d_row_slot, int32_t* d_row_expert,
                          void* d_rows, int32_t* d_status, void* d_scratch, void* stream);
+/* d_row_slot[pos[t,k]] = t*K + k, [M]; -1 for rows without a slot.
+ * No counterpart of its own in the reference (whose plan is always its own sort). */
+int bwmoe_plan_row_slots(const int32_t* d_pos, int T, int K, int32_t* d_row_slot, void* stream);
 /* d_rows[pos[t,k],:] = x[t,:].  No counterpart of its own in the reference (a gather inside permute_tokens). */
 int bwmoe_permute_rows(const void* d_x, const int32_t* d_pos, const int32_t* d_offsets, int T, int D, int E, int K,
                        int dtype, void* d_rows, void* stream);
@@ -535,8 +542,8 @@ int bwmoe_unpermute_rows_backward(const void* d_dout, const void* d_rows, const 
  *
  * bwmoe_int_quant: scale[t] = fl32(max|x[t,:]| / 127), codes = x / scale rounded to nearest, ties to even, exactly.  A
  * row of zeros gets scale 0; a row with an infinity or a NaN gets scale NaN and codes 0, which makes its products NaN.
- * With d_pos (and d_offsets) codes and scale go to the token's K rows in expert order, [T*K, D] and [T*K] (rows that no
- * slot owns: zeros); d_pos null, K = 1: in place of the token.
+ * With d_pos (and d_offsets; E = 0 and the rows' slots for other plans, as above) codes and scale go to the token's K rows in
+ * expert order, [T*K, D] and [T*K] (rows that no slot owns: zeros); d_pos null, K = 1: in place of the token.
  */
 int bwmoe_int_quant(const void* d_x, const int32_t* d_pos, const int32_t* d_offsets, int T, int D, int E, int K, int dtype,
                      void* d_codes, float* d_scales, void* stream);

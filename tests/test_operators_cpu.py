@@ -124,3 +124,16 @@ def test_sizes_past_32_bits_are_refused():
                  lambda: bw.int8_moe_forward_routed(m(4, 16), m(4, 2, dtype=F32), m(4, 2, dtype=I32), w, w, m(2, big, 16, dtype=I8), ws, ws, m(2, 16, dtype=F32))):
         with pytest.raises(ValueError, match="sizes"):
             call()
+
+
+def test_row_slots_and_negative_expert_counts_are_refused():
+    lib, p = bw.lib(), 4096
+    bad = lambda rc, code, word: rc == code and word in _lib.last_error()                    # noqa: E731
+    assert bad(lib.bwmoe_plan_row_slots(p, 0, 2, p, None), -1, "plan_row_slots")
+    assert bad(lib.bwmoe_plan_row_slots(p, 4, 33, p, None), -4, "plan_row_slots")
+    assert bad(lib.bwmoe_plan_row_slots(p, 2 ** 31 - 1, 1, p, None), -4, "too large")
+    assert bad(lib.bwmoe_plan_row_slots(None, 4, 2, p, None), -6, "plan_row_slots")
+    assert bad(lib.bwmoe_plan_row_slots(p, 4, 2, None, None), -6, "plan_row_slots")
+    assert bad(lib.bwmoe_permute_rows(p, p, p, 4, 16, -1, 2, 0, p, None), -1, "permute_rows")
+    assert bad(lib.bwmoe_unpermute_rows_backward(p, p, p, p, p, 4, 16, -1, 2, 0, p, None, None), -6, "backward")
+    assert bad(lib.bwmoe_int_quant(p, p, p, 4, 32, -1, 2, 0, p, p, None), -1, "int_quant")

@@ -375,3 +375,76 @@ def test_the_largest_number_of_rows():
     assert torch.equal(bw.unpermute_tokens(rows, plan)[:7], x[:7])
     del idx, x, rows, plan
     torch.cuda.empty_cache()
+
+
+def in_used_memory(shape, dtype, call):
+    """The call's result where the allocator hands it memory that holds NaN (in 8-bit integers: -1)."""
+    torch.cuda.synchronize()
+    block = torch.full(shape, float("nan"), dtype=dtype, device=DEV) if dtype.is_floating_point else torch.full(shape, -1, dtype=dtype, device=DEV)
+    del block
+    return call()
+
+
+@pytest.mark.parametrize("how", ["dropped", "elsewhere", "in place", "inference"])
+@pytest.mark.parametrize("T,D,E,K,dtype", [(4, 32, 2, 1, F32), (90, 1024, 16, 2, BF16), (37, 50, 8, 3, F16), (300, 2048, 32, 8, BF16), (41, 66, 64, 11, F32)])
+def test_rows_that_no_slot_of_a_plan_from_elsewhere_owns(T, D, E, K, dtype, how):
+    """Slots dropped from a plan leave rows in the middle of a segment without an owner: zeros, in every operator that writes
+    rows."""
+    idx, w = routing(T, E, K, T)
+    g = torch.Generator().manual_seed(K)
+    with torch.inference_mode(how == "inference"):
+        made = bw.permute_plan(idx.to(DEV), E)
+        gone = (torch.rand(T, K, generator=g) < 0.4).to(DEV)
+        gone[0, 0], gone[1, 0] = True, False
+        if how in ("in place", "inference"):
+            made.pos[gone] = -1
+            plan = made
+        else:
+            pos = torch.where(gone, -1, made.pos)
+            if how == "dropped":
+                plan = made._replace(pos=pos)
+            else:                                           # other segments, rows in another order, places past the rows
+                other = torch.randperm(T * K, generator=g).to(DEV, torch.int32)
+                pos = torch.where(gone, T * K + 5, other[made.pos.long()])
+                plan = bw.PermutePlan(torch.tensor([0, 3 * T * K], dtype=torch.int32, device=DEV), pos)
+        x, dout = (torch.randn(T, D, generator=g).to(dtype).to(DEV) for _ in range(2))
+        rows, _ = in_used_memory((T * K, D), dtype, lambda: bw.permute_tokens(x, plan=plan))
+        pos = plan.pos
+        owned = torch.zeros(T * K, dtype=torch.bool, device=DEV)
+        owned[pos[~gone].long()] = True
+        token = torch.arange(T, device=DEV)[:, None].expand(T, K)[~gone]
+        want = torch.zeros_like(rows)
+        want[pos[~gone].long()] = x[token]
+        assert torch.equal(rows, want)
+        wt = w.to(DEV)
+        drows, dw = in_used_memory((T * K, D), dtype, lambda: bw.unpermute_tokens_backward(dout, rows, plan, wt))
+        want[pos[~gone].long()] = (wt[~gone][:, None] * dout[token].float()).to(dtype)
+        assert torch.equal(drows, want) and (dw[gone] == 0).all() and not dw.isnan().any()
+        if D % 16 == 0:
+            alone, scale = bw.quantize_tokens_int8(x)
+            codes, scales = in_used_memory((T * K, D), torch.int8, lambda: bw.quantize_tokens_int8(x, plan))
+            want, ws = torch.zeros_like(codes), torch.zeros_like(scales)
+            want[pos[~gone].long()], ws[pos[~gone].long()] = alone[token], scale[token]
+            assert torch.equal(codes, want) and torch.equal(scales, ws)
+    if how != "inference":
+        rg = rows.detach().clone().requires_grad_()
+        d, = in_used_memory((T * K, D), dtype, lambda: torch.autograd.grad(bw.unpermute_tokens(rg, plan), rg, dout))
+        assert torch.equal(d[~owned], torch.zeros_like(d[~owned])) and torch.equal(d[pos[~gone].long()], dout[token])
+        d, = in_used_memory((T * K, D), dtype, lambda: torch.autograd.grad(bw.unpermute_tokens(rg, plan, wt), rg, dout))
+        assert torch.equal(d, drows)
+
+
+def test_the_librarys_own_plans_need_no_owners():
+    """One launch, as long as nothing was written to them."""
+    idx, _ = routing(40, 8, 2, 0)
+    x = torch.randn(40, 64, device=DEV)
+    _, plan = bw.permute_tokens(x, idx.to(DEV), 8)
+    lib = bw.lib()
+
+    def launches(p):
+        n = lib.bwmoe_launch_count()
+        bw.permute_tokens(x, plan=p)
+        return lib.bwmoe_launch_count() - n
+    assert launches(plan) == 1 and launches(bw.PermutePlan(*plan)) == 2
+    plan.pos[3, 1] = -1
+    assert launches(plan) == 2
