@@ -16,7 +16,7 @@ import functools
 import torch
 
 from . import _lib
-from .moe import _contig, _on_device, _require_cuda, _stream, _thread_workspace
+from .moe import _contig, _int32_ids, _on_device, _require_cuda, _stream, _thread_workspace
 from .permute import _DTYPES, _MAX_SIZE, _check_plan, _check_sizes, _dtype_code, _is_own, _row_owners
 
 _I8 = torch.int8
@@ -152,7 +152,7 @@ def _int8_workspace(lib, dev, T, D, H, E, K):
 def int8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, experts_w_up, experts_w_down,
                             scales_gate, scales_up, scales_down) -> torch.Tensor:
     """The block over experts in 8-bit integers, with the caller's routing (``router_weights[T,K]`` fp32,
-    ``expert_indices[T,K]`` int32): ``x[T,D]`` bf16 or fp16 -> ``out[T,D]``.  Equal, bit for bit, to
+    ``expert_indices[T,K]`` int32 or int64): ``x[T,D]`` bf16 or fp16 -> ``out[T,D]``.  Equal, bit for bit, to
     :func:`permute_tokens`' plan, :func:`quantize_tokens_int8`, :func:`int8_grouped_swiglu`, :func:`quantize_tokens_int8`,
     :func:`int8_grouped_gemm` and :func:`unpermute_tokens` in a row, every result in x's type."""
     if x.dtype not in (torch.bfloat16, torch.float16):
@@ -161,7 +161,7 @@ def int8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, e
     assert router_weights.shape == expert_indices.shape and expert_indices.dim() == 2 and expert_indices.shape[0] == T, \
         (router_weights.shape, expert_indices.shape)
     K = expert_indices.shape[1]
-    weights, indices = (_contig(t, "routing") for t in (router_weights.to(torch.float32), expert_indices.to(torch.int32)))
+    weights, indices = (_contig(t, "routing") for t in (router_weights.to(torch.float32), _int32_ids(expert_indices, E)))
     _require_cuda(x, weights, indices)
     lib = _lib.lib()
     with _on_device(dev):

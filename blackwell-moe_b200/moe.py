@@ -58,6 +58,12 @@ def _on_device(dev):
     return _SAME_DEVICE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
+def _int32_ids(ids: torch.Tensor, n: int) -> torch.Tensor:
+    """Ids of ``n`` things as the library takes them.  A 64-bit one outside 32 bits stays out of range instead of wrapping
+    around to a valid one."""
+    return (ids.clamp(-1, n) if ids.dtype == torch.int64 else ids).to(torch.int32)
+
+
 def _workspace(dev, nbytes: int) -> torch.Tensor:
     """One grow-only workspace per (device, stream): calls on one stream are
     ordered, so they can share it; different streams get their own."""
@@ -305,13 +311,14 @@ def fp8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, ex
     assert router_weights.shape == expert_indices.shape and router_weights.shape[0] == T
     K = router_weights.shape[1]
     block = scales_gate.dim() == 3
-    tensors = [_contig(t, "tensor") for t in (x, router_weights.to(torch.float32), expert_indices.to(torch.int32),
+    tensors = [_contig(t, "tensor") for t in (x, router_weights.to(torch.float32),
+                                              _int32_ids(expert_indices, E if remap is None else remap.numel()),
                                               experts_w_gate, experts_w_up, experts_w_down,
                                               scales_gate, scales_up, scales_down)]
     dev = _require_cuda(*tensors)
     n_total = 0
     if remap is not None:
-        remap = _contig(remap.to(torch.int32), "remap")
+        remap = _contig(_int32_ids(remap, E), "remap")
         _require_cuda(x, remap)
         n_total = remap.numel()
     lib = _lib.lib()
@@ -361,8 +368,8 @@ def streaming_moe_forward(x, w_gate, cache, layer_idx: int, top_k: int, prefetch
     slots = cache.fetch(layer_idx, unique_eids.tolist())
     n_total = max(int(w_gate.shape[1]), int(getattr(cache, "n_experts", 0)))
     remap = torch.full((n_total,), -1, dtype=torch.int32, device=x.device)
-    remap[unique_eids.long()] = slots.to(device=x.device, dtype=torch.int32)
     gpu = cache.gpu
+    remap[unique_eids.long()] = _int32_ids(slots.to(device=x.device), gpu["gate_q"].shape[0])
     return fp8_moe_forward_routed(x, weights, indices, gpu["gate_q"], gpu["up_q"], gpu["down_q"],
                                   gpu["scale_g"], gpu["scale_u"], gpu["scale_d"], remap=remap)
 

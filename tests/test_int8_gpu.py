@@ -597,3 +597,13 @@ def test_swiglu_is_rounded_to_16_bits_once(counts, loose, K, N):
                 bits = out[t][rows], out[F32][rows].to(t)
                 # once in a million the quotient is rounded the other way; with that, once in 2^8 or less the 16 bits
                 assert int((bits[0] != bits[1])[near].sum()) <= 1, (e, t)
+
+
+def test_ids_of_64_bits_do_not_wrap_around():
+    """2^32 + 1 is no expert, not expert 1; valid ids in 64 bits are what they are in 32."""
+    x, weights, idx, ws, ss = make_block(30, 256, 512, 8, 2, BF16, 1)
+    assert torch.equal(bw.int8_moe_forward_routed(x, weights, idx.long(), *ws, *ss), bw.int8_moe_forward_routed(x, weights, idx, *ws, *ss))
+    wide, none = idx.long(), idx.clone()
+    for t, id64 in enumerate((2 ** 32 + 1, -2 ** 32, 2 ** 40 + 3, -2 ** 63, 2 ** 63 - 1, 8, -1)):
+        wide[t, t % 2], none[t, t % 2] = id64, -1
+    assert torch.equal(bw.int8_moe_forward_routed(x, weights, wide, *ws, *ss), bw.int8_moe_forward_routed(x, weights, none, *ws, *ss))

@@ -135,3 +135,25 @@ def test_forward_on_experts_loaded_from_reference_written_files(golden):
     x, wg = from_bits(g["x"], torch.bfloat16), from_bits(g["wg"], torch.bfloat16)
     out = bw.fp8_moe_forward(x.cuda(), wg.cuda(), *W, top_k=K).cpu()
     assert oracle.rel_l1(out, from_bits(g["y_fp8"], torch.bfloat16)) < 1e-2
+
+
+@pytest.mark.parametrize("remapped", [False, True])
+def test_ids_of_64_bits_do_not_wrap_around(remapped):
+    """2^32 + 1 is no expert, not expert 1, neither as an id nor as a slot that a remap table names."""
+    import blackwell_moe_b200 as bw
+    T, D, E, K, H = 40, 256, 8, 2, 128
+    c = to_cuda(make_inputs(T, D, E, K, H, seed=54, keep_bf16=False))
+    w, idx = bw.top_k_router(c["x"], c["w_gate"], K)
+    pool = [c[k] for k in ("q_gate", "q_up", "q_down", "s_gate", "s_up", "s_down")]
+    table = torch.arange(E, device="cuda:0") if remapped else None
+    call = lambda ids, remap=table: bw.fp8_moe_forward_routed(c["x"], w, ids, *pool, remap=remap)       # noqa: E731
+    assert torch.equal(call(idx.long()), call(idx))
+    wide, none = idx.long(), idx.clone()
+    for t, id64 in enumerate((2 ** 32 + 1, -2 ** 32, 2 ** 63 - 1, E, -1)):
+        wide[t, t % 2], none[t, t % 2] = id64, -1
+    assert torch.equal(call(wide), call(none))
+    if remapped:
+        holes = table.clone()
+        holes[3], wide = -1, table.clone()
+        wide[3] = 2 ** 32 + 5
+        assert torch.equal(call(idx, wide), call(idx, holes))
