@@ -16,7 +16,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .moe import (_contig, _require_cuda, _stream, _workspace, fp8_moe_forward, fp8_moe_forward_shared,
+from .moe import (_contig, _exclusive, _require_cuda, _stream, _workspace, fp8_moe_forward, fp8_moe_forward_shared,
                   stack_shared_experts)
 from .quant import quant_fp8_e4m3
 
@@ -34,7 +34,7 @@ def fp8_dense_mlp(x, w_gate, w_up, w_down, s_gate, s_up, s_down) -> torch.Tensor
     ss = [s.reshape(1).to(torch.float32).contiguous() for s in (s_gate, s_up, s_down)]
     dev = _require_cuda(*ts, *ss)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
+    with torch.cuda.device(dev), _exclusive(dev):
         need = lib.bwmoe_workspace_bytes(T, D, H, 1, 1)
         if need == 0:
             raise ValueError(f"unsupported shape T={T} D={D} H={H}")

@@ -64,9 +64,22 @@ def _int32_ids(ids: torch.Tensor, n: int) -> torch.Tensor:
     return (ids.clamp(-1, n) if ids.dtype == torch.int64 else ids).to(torch.int32)
 
 
+_workspace_locks: dict = {}
+
+
+def _exclusive(dev):
+    """The lock of the current stream's workspace.  A call holds it from asking for the workspace to its last launch:
+    the launches of one call are ordered behind those of another, but two threads' would interleave."""
+    key = (dev.index, _stream(dev))
+    return _workspace_locks.get(key) or _workspace_locks.setdefault(key, threading.RLock())
+
+
 def _workspace(dev, nbytes: int) -> torch.Tensor:
     """One grow-only workspace per (device, stream): calls on one stream are
-    ordered, so they can share it; different streams get their own."""
+    ordered (see :func:`_exclusive`), so they can share it; different streams get their own.
+    During capture one of the graph's own, so that graphs replayed side by side share nothing."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
     key = (dev.index, _stream(dev))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
@@ -188,7 +201,7 @@ def fp8_moe_forward(x, w_gate, experts_w_gate, experts_w_up, experts_w_down,
     dev = _require_cuda(*weights)
     lib = _lib.lib()
     x = _contig(x, "x")
-    with _on_device(dev):
+    with _on_device(dev), _exclusive(dev):
         ptrs = [t.data_ptr() for t in weights]
         if routed_scale != 1.0 or residual is not None:
             if scales_gate.dim() == 3 or not x.is_cuda:
@@ -261,7 +274,7 @@ def fp8_moe_forward_shared(x, w_gate, experts_w_gate, experts_w_up, experts_w_do
                                               scales_gate, scales_up, scales_down)]
     dev = _require_cuda(*tensors)
     lib = _lib.lib()
-    with _on_device(dev):
+    with _on_device(dev), _exclusive(dev):
         need = lib.bwmoe_workspace_bytes_shared(T, D, H, E, top_k, n_shared)
         if need == 0:
             raise ValueError(f"unsupported shape T={T} D={D} H={H} E={E}+{n_shared} top_k={top_k}+{n_shared}")
@@ -322,7 +335,7 @@ def fp8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, ex
         _require_cuda(x, remap)
         n_total = remap.numel()
     lib = _lib.lib()
-    with _on_device(dev):
+    with _on_device(dev), _exclusive(dev):
         need = (lib.bwmoe_workspace_bytes_block if block else lib.bwmoe_workspace_bytes)(T, D, H, E, K)
         if need == 0:
             raise ValueError(f"unsupported shape T={T} D={D} H={H} E={E} top_k={K}")
@@ -390,7 +403,8 @@ _TENSOR_ONLY = ("scale_x", "scale_h", "h")
 def moe_stage_views(dev, T: int, D: int, H: int, E: int, K: int, block: bool = False) -> dict:
     """Copies of the intermediates the last forward of this shape on the current
     stream left in its workspace (routing, permutation, FP8 codes, scales) and
-    the device status word.  For stage-level checks; synchronises."""
+    the device status word.  For stage-level checks; synchronises.  (Not of a captured
+    forward: its workspace is the graph's.)"""
     dev = torch.device(dev)
     lib = _lib.lib()
     ws = _workspaces[(dev.index, _stream(dev))]

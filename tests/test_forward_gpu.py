@@ -224,3 +224,81 @@ def test_down_projection_on_cta_pairs_equals_single_cta_tiles():
         rows = slice(seg[e], seg[e + 1])
         ref[rows] = (hq[rows].float() @ wd[e].float()) / (sh[e] * sd[e])
     assert oracle.rel_l1(outs[0].float().cpu(), ref.cpu()) < 5e-3
+
+
+def _forwards(T, seed):
+    """Calls of every forward that takes a workspace of the package's, on inputs of their own."""
+    import blackwell_moe_b200 as bw
+    D, E, K, H = 256, 8, 2, 256
+    c = to_cuda(make_inputs(T, D, E, K, H, seed=seed, keep_bf16=False))
+    g = torch.Generator(device="cuda:0").manual_seed(seed)
+    inv = [torch.rand(E, a // 128, b // 128, generator=g, device="cuda:0") * 1e-2 for a, b in ((D, H), (D, H), (H, D))]
+    q, s = [c["q_" + k] for k in ("gate", "up", "down")], [c["s_" + k] for k in ("gate", "up", "down")]
+    w, idx = bw.top_k_router(c["x"], c["w_gate"], K)
+    routed = c["w_gate"][:, :E - 1].contiguous()
+    return [lambda: bw.fp8_moe_forward(c["x"], c["w_gate"], *q, *s, top_k=K),
+            lambda: bw.fp8_moe_forward(c["x"], c["w_gate"], *q, *inv, top_k=K),
+            lambda: bw.fp8_moe_forward(c["x"], c["w_gate"], *q, *s, top_k=K, routed_scale=1.5, residual=c["x"]),
+            lambda: bw.fp8_moe_forward_routed(c["x"], w, idx, *q, *s),
+            lambda: bw.fp8_moe_forward_routed(c["x"], w, idx, *q, *inv),
+            lambda: bw.fp8_moe_forward_shared(c["x"], routed, *q, *s, top_k=K, n_shared=1),
+            lambda: bw.fp8_dense_mlp(c["x"], *[t[0] for t in q], *[t[0] for t in s])]
+
+
+def test_two_threads_on_one_stream():
+    """Calls are several launches: those of two threads must not interleave where they share the stream's workspace."""
+    import threading
+    sets = [_forwards(T, T) for T in (5, 300)]
+    want = [[f() for f in fs] for fs in sets]
+    torch.cuda.synchronize()
+    got, threads = [[], []], []
+    for i, fs in enumerate(sets):
+        threads.append(threading.Thread(target=lambda i=i, fs=fs: [got[i].append([f() for f in fs]) for _ in range(60)]))
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for outs, ref in zip(got, want):
+        assert len(outs) == 60 and all(torch.equal(a, b) for out in outs for a, b in zip(out, ref))
+
+
+@pytest.mark.parametrize("T", [5, 300])
+def test_graphs_that_are_replayed_side_by_side(T):
+    """Two graphs captured on one stream, replayed on two at once: they have no workspace in common, and a plain call beside them
+    has its own."""
+    sets = [_forwards(T, seed) for seed in (1, 2, 3)]
+    want = [[f() for f in fs] for fs in sets]
+    graphs, outs = [], []
+    for fs in sets[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append([f() for f in fs])
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        plain = [f() for f in sets[2]]
+    torch.cuda.synchronize()
+    for got, ref in zip([*outs, plain], want):
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_a_captured_forward_takes_memory_of_its_graph():
+    """While a graph is captured the stream's own workspace is neither used nor replaced."""
+    import blackwell_moe_b200 as bw
+    fs = _forwards(40, 7)
+    fs[0]()
+    key = (0, torch.cuda.current_stream().cuda_stream)
+    mine = bw.moe._workspaces[key]
+    mine.fill_(0x55)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fs[0]()
+    before = dict(bw.moe._workspaces)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bw.moe._workspaces[key] is mine and bool((mine == 0x55).all()) and before.keys() == bw.moe._workspaces.keys()
+    assert torch.equal(out, fs[0]())
