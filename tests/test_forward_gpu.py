@@ -289,13 +289,15 @@ def test_graphs_that_are_replayed_side_by_side(T):
 def test_a_captured_forward_takes_memory_of_its_graph():
     """While a graph is captured the stream's own workspace is neither used nor replaced."""
     import blackwell_moe_b200 as bw
-    fs = _forwards(40, 7)
-    fs[0]()
-    key = (0, torch.cuda.current_stream().cuda_stream)
-    mine = bw.moe._workspaces[key]
-    mine.fill_(0x55)
+    fs, stream = _forwards(40, 7), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    key = (0, stream.cuda_stream)
+    with torch.cuda.stream(stream):
+        fs[0]()
+        mine = bw.moe._workspaces[key]
+        mine.fill_(0x55)
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.cuda.graph(graph, stream=stream):
         out = fs[0]()
     before = dict(bw.moe._workspaces)
     graph.replay()
