@@ -3,7 +3,8 @@
 ``value = code * scale`` on both sides.  Weights keep the package's ``[E, in, out]`` layout, int8, with scales
 ``[E, out]`` fp32 (``quantize_expert_weights_int8`` makes them at load time); activations are quantised token by token
 on every call.  The products are summed in 32-bit integers, exactly, on the tensor cores, so a token's result does not
-depend on the batch around it.  Inference only: no gradients.
+depend on the batch around it.  Inference only: the operators have no derivative, and a backward pass that reaches one
+raises.
 
 The reference has no counterpart (its integer path, src/blackwell_moe/kernels/int4_moe.py, is 4-bit and weights only);
 ``int8_moe_forward`` keeps the argument order of ``fp8_moe_forward`` (src/blackwell_moe/kernels/fp8_moe.py:111-121).
@@ -12,14 +13,53 @@ The reference has no counterpart (its integer path, src/blackwell_moe/kernels/in
 from __future__ import annotations
 
 import functools
+import inspect
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .moe import _contig, _int32_ids, _on_device, _require_cuda, _stream, _thread_workspace
-from .permute import _DTYPES, _MAX_SIZE, _check_plan, _check_sizes, _dtype_code, _is_own, _row_owners
+from .permute import _DTYPES, _MAX_SIZE, _check_plan, _check_sizes, _dtype_code, _has_tangent, _is_own, _row_owners
 
 _I8 = torch.int8
+
+
+class _WithoutDerivative(torch.autograd.Function):
+    """A call among differentiable ones.  Without a node of its own its result would look like a constant, and the gradients of
+    what is in front of it would be wrong without a word."""
+
+    @staticmethod
+    def forward(ctx, fn, *args):
+        ctx.name = fn.__name__
+        return fn(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(f"{ctx.name} has no gradient: call it under torch.no_grad(), or with detached tensors")
+
+
+def _inference_only(fn):
+    signature = inspect.signature(fn)
+
+    def checked(args, kwargs):
+        tensors = [a for a in (*args, *kwargs.values()) if isinstance(a, torch.Tensor)]
+        if (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or (forward_ad._current_level >= 0 and _has_tangent(*tensors)):
+            bound = signature.bind(*args, **kwargs)
+            bound.apply_defaults()
+            return _WithoutDerivative.apply(fn, *bound.args)
+        return fn(*args, **kwargs)
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        for a in args:                       # (the usual call at a third of the cost: small products are bound by the host)
+            if getattr(a, "requires_grad", False):
+                break
+        else:
+            if forward_ad._current_level < 0 and not any(getattr(a, "requires_grad", False) for a in kwargs.values()):
+                return fn(*args, **kwargs)
+        return checked(args, kwargs)
+    return call
 
 
 def _out_code(dtype) -> int:
@@ -28,6 +68,7 @@ def _out_code(dtype) -> int:
     return _DTYPES[dtype]
 
 
+@_inference_only
 def quantize_tokens_int8(x: torch.Tensor, plan=None):
     """``x[T,D]`` (bf16, fp16 or fp32; D a multiple of 16) -> ``(codes[T,D] int8, scales[T] fp32)``:
     ``scale = max|x| / 127`` of the row, codes rounded to nearest, ties to even.  A row of zeros has scale 0; a row with an
@@ -88,12 +129,14 @@ def _grouped(fn_name, codes, scales, offsets, weights, w_scales, out_dtype):
     return out
 
 
+@_inference_only
 def int8_grouped_gemm(codes, scales, offsets, w, w_scales, out_dtype=torch.bfloat16) -> torch.Tensor:
     """``out[M,N]``: the rows ``offsets[e] .. offsets[e+1]-1`` of ``codes[M,K]`` int8 (scales ``[M]``) times ``w[e]`` of
     ``w[E,K,N]`` int8 (scales ``[E,N]``); K and N multiples of 16.  Rows of no segment are zero."""
     return _grouped("bwmoe_int_grouped_gemm", codes, scales, offsets, (w,), (w_scales,), out_dtype)
 
 
+@_inference_only
 def int8_grouped_swiglu(codes, scales, offsets, w_gate, w_up, s_gate, s_up, out_dtype=torch.bfloat16) -> torch.Tensor:
     """``silu(gate) * up`` of the two grouped products with ``w_gate`` and ``w_up``, in one pass over the rows."""
     return _grouped("bwmoe_int_gateup_swiglu", codes, scales, offsets, (w_gate, w_up), (s_gate, s_up), out_dtype)
@@ -104,6 +147,7 @@ def _matmul_workspace_bytes(device_index, T, K, N):         # (sizes go by the d
     return _lib.lib().bwmoe_workspace_bytes_int_matmul(T, K, N)
 
 
+@_inference_only
 def int8_matmul(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
     """``x[T,K]`` (bf16, fp16 or fp32), quantised token by token, times ``w[K,N]`` int8 with scales ``[N]``, in x's type."""
     assert x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[0], (x.shape, w.shape)
@@ -149,6 +193,7 @@ def _int8_workspace(lib, dev, T, D, H, E, K):
     return _thread_workspace(dev, need)
 
 
+@_inference_only
 def int8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, experts_w_up, experts_w_down,
                             scales_gate, scales_up, scales_down) -> torch.Tensor:
     """The block over experts in 8-bit integers, with the caller's routing (``router_weights[T,K]`` fp32,
@@ -176,6 +221,7 @@ def int8_moe_forward_routed(x, router_weights, expert_indices, experts_w_gate, e
     return out
 
 
+@_inference_only
 def int8_moe_forward(x, w_gate, experts_w_gate, experts_w_up, experts_w_down, scales_gate, scales_up, scales_down,
                      top_k: int = 8) -> torch.Tensor:
     """:func:`int8_moe_forward_routed` behind :func:`top_k_router`: ``x[T,D]`` bf16, ``w_gate[D,E]`` bf16."""

@@ -607,3 +607,31 @@ def test_ids_of_64_bits_do_not_wrap_around():
     for t, id64 in enumerate((2 ** 32 + 1, -2 ** 32, 2 ** 40 + 3, -2 ** 63, 2 ** 63 - 1, 8, -1)):
         wide[t, t % 2], none[t, t % 2] = id64, -1
     assert torch.equal(bw.int8_moe_forward_routed(x, weights, wide, *ws, *ss), bw.int8_moe_forward_routed(x, weights, none, *ws, *ss))
+
+
+def test_a_backward_pass_through_the_integers_says_that_there_is_none():
+    """The operators stand among differentiable ones: a gradient that ends in them must not do so silently."""
+    from torch.autograd import forward_ad as fw
+    x, weights, idx, (wg, wu, wd), (sg, su, sd) = make_block(6, 64, 64, 4, 2, BF16, 0)
+    gate = torch.randn(64, 4, device=DEV).to(BF16)
+    rows, plan = bw.permute_tokens(x, idx, 4)
+    codes, s = bw.quantize_tokens_int8(rows)
+    calls = [(lambda x: bw.quantize_tokens_int8(x)[1], x), (lambda x: bw.quantize_tokens_int8(x, plan)[1], x),
+             (lambda s: bw.int8_grouped_gemm(codes, s, plan.offsets, wg, sg), s), (lambda sg: bw.int8_grouped_gemm(codes, s, plan.offsets, wg, w_scales=sg), sg),
+             (lambda s: bw.int8_grouped_swiglu(codes, s, plan.offsets, wg, wu, sg, su, out_dtype=F32), s),
+             (lambda x: bw.int8_matmul(x, wg[0], sg[0]), x), (lambda x: bw.int8_moe_forward_routed(x, weights, idx, wg, wu, wd, sg, su, sd), x),
+             (lambda w: bw.int8_moe_forward_routed(x, w, idx, wg, wu, wd, sg, su, scales_down=sd), weights),
+             (lambda x: bw.int8_moe_forward(x, gate, wg, wu, wd, sg, su, sd, top_k=2), x)]
+    for call, t in calls:
+        want, leaf = call(t), t.clone().requires_grad_()
+        out = call(leaf)
+        assert torch.equal(out.detach(), want) and not want.requires_grad
+        with pytest.raises(NotImplementedError, match="has no gradient"):
+            (leaf.float().sum() + out.float().sum()).backward()
+        with torch.no_grad():
+            assert torch.equal(call(leaf), want) and not call(leaf).requires_grad
+        with fw.dual_level():
+            with pytest.raises(NotImplementedError):
+                call(fw.make_dual(t, torch.ones_like(t)))
+            assert torch.equal(call(t), want)
+    assert not bw.quantize_tokens_int8(x.clone().requires_grad_())[0].requires_grad
