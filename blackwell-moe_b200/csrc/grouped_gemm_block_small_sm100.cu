@@ -329,23 +329,6 @@ block_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
 }
 
-// activations [rows, kdim] e4m3 row-major: box 128 (K) x 32 (rows), 128-byte swizzle
-int make_map_x32(CUtensorMap* map, const void* base, int rows, int kdim) {
-  if (tensor_map_lookup(2, base, rows, kdim, 0, map)) return BWMOE_OK;
-  auto fn = encode_fn();
-  BWMOE_REQUIRE(fn != nullptr, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
-  cuuint64_t dims[2] = {(cuuint64_t)kdim, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)kdim};
-  cuuint32_t box[2] = {BK, S_NT};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  BWMOE_REQUIRE(r == CUDA_SUCCESS, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled(X: rows=%d k=%d) failed: %d", rows, kdim, (int)r);
-  tensor_map_store(2, base, rows, kdim, 0, *map);
-  return BWMOE_OK;
-}
-
 template <bool GATE_UP>
 int launch_small(const CUtensorMap& mx, const CUtensorMap& mw0, const CUtensorMap& mw1, const SmallParams& p, int M,
                  cudaStream_t st) {
@@ -369,7 +352,7 @@ int launch_gateup_block_small(const void* xq, const float* x_inv, const int32_t*
                               const float* inv_g, const float* inv_u, int M, int D, int H, int E, void* hq,
                               float* h_inv, int32_t* status, cudaStream_t st) {
   CUtensorMap mx, mg, mu;
-  if (int rc = make_map_x32(&mx, xq, M, D)) return rc;
+  if (int rc = make_map_rows(&mx, xq, M, D, S_NT)) return rc;
   if (int rc = make_map_b(&mg, wg, E, D, H)) return rc;
   if (int rc = make_map_b(&mu, wu, E, D, H)) return rc;
   SmallParams p{offsets, x_inv, inv_g, inv_u, hq, h_inv, status, E, H, ceil_div(H, BN_HALF), ceil_div(D, BK),
@@ -380,7 +363,7 @@ int launch_gateup_block_small(const void* xq, const float* x_inv, const int32_t*
 int launch_down_block_small(const void* hq, const float* h_inv, const int32_t* offsets, const void* wd,
                             const float* inv_d, int M, int D, int H, int E, void* y, int32_t* status, cudaStream_t st) {
   CUtensorMap mx, mw;
-  if (int rc = make_map_x32(&mx, hq, M, H)) return rc;
+  if (int rc = make_map_rows(&mx, hq, M, H, S_NT)) return rc;
   if (int rc = make_map_b(&mw, wd, E, H, D)) return rc;
   SmallParams p{offsets, h_inv, inv_d, nullptr, y, nullptr, status, E, D, ceil_div(D, 2 * BN_HALF), ceil_div(H, BK),
                 ceil_div(D, 128)};

@@ -721,23 +721,6 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
 }
 
-// rows [rows, kdim] of 8-bit integers: box 128 (K) x 32 (rows), 128-byte swizzle (kind 2: the map of the block-scale kernel's rows)
-int make_map_rows32(CUtensorMap* map, const void* base, int rows, int kdim) {
-  if (tensor_map_lookup(2, base, rows, kdim, 0, map)) return BWMOE_OK;
-  auto fn = encode_fn();
-  BWMOE_REQUIRE(fn != nullptr, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
-  cuuint64_t dims[2] = {(cuuint64_t)kdim, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)kdim};
-  cuuint32_t box[2] = {BK, 32};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  BWMOE_REQUIRE(r == CUDA_SUCCESS, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled(rows=%d k=%d) failed: %d", rows, kdim, (int)r);
-  tensor_map_store(2, base, rows, kdim, 0, *map);
-  return BWMOE_OK;
-}
-
 // Which kernel a product gets.  32-row tiles: few rows per expert, or tiles so few that they fit the SMs at once (and K blocks
 // few enough that reading the weights again for every 32 rows does not count).  Measured, us, 32-row tiles against 128-row tiles
 // (launched one after the other, weights from memory):
@@ -894,7 +877,7 @@ int launch_int8_gemm(const void* a, const float* row_scale, const int32_t* offse
   const int n_tiles = ceil_div(N, swiglu ? BN_HALF : BN);
   const bool small = small_applies(M, K, n_tiles, E);
   CUtensorMap ma, mb0, mb1;
-  if (int rc = small ? make_map_rows32(&ma, a, M, K) : make_map_a(&ma, a, M, K)) return rc;
+  if (int rc = small ? make_map_rows(&ma, a, M, K, S_NT) : make_map_a(&ma, a, M, K)) return rc;
   if (int rc = make_map_b(&mb0, w0, E, K, N)) return rc;
   if (int rc = make_map_b(&mb1, swiglu ? w1 : w0, E, K, N)) return rc;
   I8Params p{offsets, row_scale, scale0, scale1, out, status, E, M, K, N, n_tiles, early && !clear,

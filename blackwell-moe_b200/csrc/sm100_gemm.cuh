@@ -331,23 +331,24 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 bool tensor_map_lookup(int kind, const void* base, int d0, int d1, int d2, CUtensorMap* out);
 void tensor_map_store(int kind, const void* base, int d0, int d1, int d2, const CUtensorMap& map);
 
-// activations [rows, kdim] e4m3 row-major: box 128 (K) x 128 (rows), 128-byte swizzle
-inline int make_map_a(CUtensorMap* map, const void* base, int rows, int kdim) {
-  if (tensor_map_lookup(0, base, rows, kdim, 0, map)) return BWMOE_OK;
+// activations [rows, kdim] of 8 bits, row-major: box 128 (K) x box_rows, 128-byte swizzle
+inline int make_map_rows(CUtensorMap* map, const void* base, int rows, int kdim, int box_rows) {
+  if (tensor_map_lookup(0, base, rows, kdim, box_rows, map)) return BWMOE_OK;
   auto fn = encode_fn();
   BWMOE_REQUIRE(fn != nullptr, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
   cuuint64_t dims[2] = {(cuuint64_t)kdim, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)kdim};
-  cuuint32_t box[2] = {BK, BM};
+  cuuint32_t box[2] = {BK, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  BWMOE_REQUIRE(r == CUDA_SUCCESS, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled(A: rows=%d k=%d) failed: %d", rows,
+  BWMOE_REQUIRE(r == CUDA_SUCCESS, BWMOE_ERR_CUDA, "cuTensorMapEncodeTiled(rows=%d k=%d) failed: %d", rows,
                 kdim, (int)r);
-  tensor_map_store(0, base, rows, kdim, 0, *map);
+  tensor_map_store(0, base, rows, kdim, box_rows, *map);
   return BWMOE_OK;
 }
+inline int make_map_a(CUtensorMap* map, const void* base, int rows, int kdim) { return make_map_rows(map, base, rows, kdim, BM); }
 // weights [E, kdim, n] e4m3, n contiguous: box 128 (N) x 128 (K) x 1, 128-byte swizzle
 inline int make_map_b(CUtensorMap* map, const void* base, int E, int kdim, int n) {
   if (tensor_map_lookup(1, base, E, kdim, n, map)) return BWMOE_OK;

@@ -635,3 +635,18 @@ def test_a_backward_pass_through_the_integers_says_that_there_is_none():
                 call(fw.make_dual(t, torch.ones_like(t)))
             assert torch.equal(call(t), want)
     assert not bw.quantize_tokens_int8(x.clone().requires_grad_())[0].requires_grad
+
+
+def test_the_same_rows_in_tiles_of_both_heights():
+    """One tensor of codes, read by the kernel of 32-row tiles and by that of 128-row tiles in turn: the descriptors of its rows
+    are kept by address and shape, and by the tile's height."""
+    M, K = 300, 512
+    a, rs = make_codes((M, K), 1).to(DEV), torch.ones(M, device=DEV)
+    few, many = make_codes((16, K, 256), 2).to(DEV), make_codes((1, K, 16384), 3).to(DEV)
+    bounds = [19 * e for e in range(16)] + [M]
+    for _ in range(2):
+        out = bw.int8_grouped_gemm(a, rs, torch.tensor(bounds, dtype=torch.int32, device=DEV), few, torch.ones(16, 256, device=DEV), out_dtype=F32)
+        for e in range(16):
+            assert torch.equal(out[bounds[e]:bounds[e + 1]].double(), a[bounds[e]:bounds[e + 1]].double() @ few[e].double())
+        out = bw.int8_grouped_gemm(a, rs, torch.tensor([0, M], dtype=torch.int32, device=DEV), many, torch.ones(1, 16384, device=DEV), out_dtype=F32)
+        assert torch.equal(out.double(), a.double() @ many[0].double())
