@@ -650,3 +650,100 @@ def test_the_same_rows_in_tiles_of_both_heights():
             assert torch.equal(out[bounds[e]:bounds[e + 1]].double(), a[bounds[e]:bounds[e + 1]].double() @ few[e].double())
         out = bw.int8_grouped_gemm(a, rs, torch.tensor([0, M], dtype=torch.int32, device=DEV), many, torch.ones(1, 16384, device=DEV), out_dtype=F32)
         assert torch.equal(out.double(), a.double() @ many[0].double())
+
+
+def check_rows_against_64_bits(out, rows_of, a, rs, offsets, ws, ss, dtype):
+    """Rows rows_of(lo, hi) of each segment against the definition: one product, or SwiGLU of two."""
+    for e in range(len(offsets) - 1):
+        rows = rows_of(offsets[e], offsets[e + 1])
+        if not len(rows):
+            continue
+        x, r = a[rows].double(), rs[rows, None].double()
+        products = [(x @ w[e].double()) * r * s[e].double() for w, s in zip(ws, ss)]
+        if len(products) == 2:
+            ref, bound = swiglu_bound(*products, dtype)
+        else:
+            ref, bound = products[0], products[0].abs() * (3.01 * U32 + half_step(dtype) * 1.001) + smallest_step(dtype)
+        assert ((out[rows].double() - ref).abs() <= bound).all(), e
+
+
+def random_product(counts, loose, K, N, swiglu, seed=9):
+    M, E = sum(counts) + loose, len(counts)
+    offsets, _ = make_segments(counts, M)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    codes = lambda *shape: torch.randint(-128, 128, shape, generator=g, device=DEV, dtype=torch.int16).to(I8)     # noqa: E731
+    a, ws = codes(M, K), [codes(E, K, N) for _ in range(1 + swiglu)]
+    rs = torch.rand(M, generator=g, device=DEV) * 1e-2
+    ss = [torch.rand(E, N, generator=g, device=DEV) * 2e-2 / K ** 0.5 for _ in ws]
+    return a, rs, offsets, ws, ss
+
+
+def product(a, rs, offsets, ws, ss, dtype):
+    call = bw.int8_grouped_swiglu if len(ws) == 2 else bw.int8_grouped_gemm
+    return call(a, rs, offsets.to(DEV), *ws, *ss, out_dtype=dtype)
+
+
+# (rows of each expert, rows of none, K, N, SwiGLU): 128-row tiles so few, and K so long, that their K loops are cut on 148 SMs - into
+# 3, 2, 2 and 5 slices, and into 2, 3 and 2 with two products; the last tiles of some have one weight box, or one that hangs over N
+CUT = [([256], 0, 14336, 4096, False), ([300], 0, 8192, 3984, False), ([200, 0, 130], 5, 8192, 3216, False), ([256], 0, 14336, 2064, False),
+       ([300], 0, 8192, 2048, True), ([300], 9, 14336, 1488, True), ([250, 3, 140], 0, 12288, 1040, True)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("counts,loose,K,N,swiglu", CUT)
+def test_cut_tiles_of_128_rows(counts, loose, K, N, swiglu, dtype):
+    case = random_product(counts, loose, K, N, swiglu)
+    out = product(*case, dtype)
+    a, rs, offsets, ws, ss = case
+    check_rows_against_64_bits(out, lambda lo, hi: list(range(lo, hi)), a, rs, offsets.tolist(), ws, ss, dtype)
+    assert (out[sum(counts):] == 0).all()
+
+
+def test_cut_tiles_one_after_the_other():
+    """Products of other tiles and slices in a row, with the slabs and counters that the one before left; twice each, and
+    inside a graph."""
+    cases = [random_product(*c) for c in CUT]
+    first = [product(*c, F32) for c in cases]
+    again = [product(*c, F32) for c in cases for _ in range(2)]
+    assert all(torch.equal(x, first[i // 2]) for i, x in enumerate(again))
+    graph = torch.cuda.CUDAGraph()
+    dev = [(a, rs, offsets.to(DEV), ws, ss) for a, rs, offsets, ws, ss in cases]
+    with torch.cuda.graph(graph):
+        captured = [product(*c, F32) for c in dev]
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(captured, first))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("counts,loose,K,N,swiglu", [([5000, 4000], 7, 4096, 8192, False), ([5000, 4000], 7, 4096, 8192, True), ([4200], 0, 8192, 5904, True),
+                                                     ([2100, 2200], 3, 4096, 12304, True), ([8200], 0, 8192, 6144, False)])
+def test_long_products_in_every_type(counts, loose, K, N, swiglu, dtype):
+    """CTA pairs; with SwiGLU also where the last weight box of a pair's tile hangs over N."""
+    a, rs, offsets, ws, ss = random_product(counts, loose, K, N, swiglu)
+    out = product(a, rs, offsets, ws, ss, dtype)
+    ends = lambda lo, hi: sorted({r for r in (lo, lo + 1, lo + 127, lo + 128, lo + 255, lo + 256, (lo + hi) // 2, hi - 129, hi - 2, hi - 1) if lo <= r < hi})      # noqa: E731
+    check_rows_against_64_bits(out, ends, a, rs, offsets.tolist(), ws, ss, dtype)
+    assert (out[sum(counts):] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,code", [(BF16, 0), (F16, 1), (F32, 2)])
+@pytest.mark.parametrize("counts,loose,K,N,swiglu", [([3, 20], 1, 256, 272, False), ([200, 150], 3, 256, 272, False), ([200, 150], 3, 256, 272, True),
+                                                     ([256], 0, 14336, 2064, False), ([5000, 4000], 7, 4096, 8192, False)])
+def test_results_at_16_byte_aligned_addresses(counts, loose, K, N, swiglu, dtype, code):
+    """Through the C entries a result may lie at any multiple of 16 bytes: nothing around it is written."""
+    from blackwell_moe_b200 import _lib
+    lib = bw.lib()
+    a, rs, offsets, ws, ss = random_product(counts, loose, K, N, swiglu)
+    offsets = offsets.to(DEV)
+    want, (M, E) = product(a, rs, offsets, ws, ss, dtype), (a.shape[0], len(counts))
+    n = lib.bwmoe_int_scratch_bytes(M, K, N, E)
+    scratch = torch.empty(n, dtype=torch.uint8, device=DEV)
+    pad = 16 * 8 // torch.finfo(dtype).bits
+    space = torch.full((M * N + 2 * pad,), 7.0, dtype=dtype, device=DEV)
+    fn = lib.bwmoe_int_gateup_swiglu if swiglu else lib.bwmoe_int_grouped_gemm
+    _lib.check(fn(a.data_ptr(), rs.data_ptr(), offsets.data_ptr(), *[w.data_ptr() for w in ws], *[s.data_ptr() for s in ss], M, K, N, E,
+                  code, space.data_ptr() + 16, scratch.data_ptr(), n, torch.cuda.current_stream().cuda_stream))
+    assert space.data_ptr() % 32 == 0
+    assert torch.equal(space[pad:-pad].view(M, N), want) and (space[:pad] == 7).all() and (space[-pad:] == 7).all()
