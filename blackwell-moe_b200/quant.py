@@ -58,12 +58,15 @@ def quantize_expert_weights_block(w: torch.Tensor):
 
 def quant_int8_channels(w: torch.Tensor):
     """8-bit integers with one scale for each output channel of ``w[..., in, out]``: ``(codes int8, scales[..., out] fp32)``
-    with ``codes * scales ~= w``; codes in [-127, 127], a channel of zeros has scale 0."""
+    with ``codes * scales ~= w``; codes in [-127, 127], a channel of zeros has scale 0.  A channel
+    with an infinity or a NaN has no representation: scale NaN, codes 0, as a row of activations."""
     wf = w.to(torch.float32)
     amax = wf.abs().amax(dim=-2)
     scales = amax / torch.full_like(amax, 127.0)       # tensor / tensor: an IEEE division on every device
+    none = ~scales.isfinite()
     safe = torch.where(scales > 0, scales, torch.ones_like(scales))
-    return torch.round(wf / safe.unsqueeze(-2)).clamp_(-127, 127).to(torch.int8), scales
+    codes = torch.round(wf / safe.unsqueeze(-2)).clamp_(-127, 127).masked_fill_(none.unsqueeze(-2), 0.0)
+    return codes.to(torch.int8), scales.masked_fill_(none, float("nan"))
 
 
 def quantize_expert_weights_int8(w: torch.Tensor):

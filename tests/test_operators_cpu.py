@@ -137,3 +137,15 @@ def test_row_slots_and_negative_expert_counts_are_refused():
     assert bad(lib.bwmoe_permute_rows(p, p, p, 4, 16, -1, 2, 0, p, None), -1, "permute_rows")
     assert bad(lib.bwmoe_unpermute_rows_backward(p, p, p, p, p, 4, 16, -1, 2, 0, p, None, None), -6, "backward")
     assert bad(lib.bwmoe_int_quant(p, p, p, 4, 32, -1, 2, 0, p, p, None), -1, "int_quant")
+
+
+def test_channels_without_a_representation():
+    w = torch.randn(2, 32, 16, generator=torch.Generator().manual_seed(1))
+    want = bw.quantize_expert_weights_int8(w)
+    bad = w.clone()
+    bad[0, 3, 1], bad[0, 4, 2], bad[1, 5, 3], bad[1, 6, 3] = float("nan"), float("inf"), -float("inf"), float("nan")
+    codes, scales = bw.quantize_expert_weights_int8(bad)
+    none = torch.zeros(2, 16, dtype=torch.bool)
+    none[0, 1] = none[0, 2] = none[1, 3] = True
+    assert torch.equal(scales.isnan(), none) and torch.equal(scales[~none], want[1][~none])
+    assert (codes.transpose(1, 2)[none] == 0).all() and torch.equal(codes.transpose(1, 2)[~none], want[0].transpose(1, 2)[~none])
