@@ -321,7 +321,8 @@ int for_type_and_piece(int dtype, int bytes, F fn) {
 }  // namespace
 
 int launch_row_slots(const int32_t* pos, int T, int K, int32_t* row_slot, cudaStream_t st) {
-  if (int rc = check_rows("plan_row_slots", T, 1, K, BWMOE_F32)) return rc;
+  BWMOE_REQUIRE(T > 0 && K > 0, BWMOE_ERR_BAD_SHAPE, "plan_row_slots: T=%d K=%d", T, K);
+  BWMOE_REQUIRE((long long)T * K <= kMaxRows, BWMOE_ERR_UNSUPPORTED, "plan_row_slots: T*K too large");
   BWMOE_REQUIRE(pos && row_slot, BWMOE_ERR_NULL, "plan_row_slots: null pointer");
   BWMOE_CUDA_OK(cudaMemsetAsync(row_slot, 0xff, sizeof(int32_t) * (size_t)T * K, st));
   BWMOE_CUDA_OK(launch_chained(row_slots_kernel, dim3((unsigned)ceil_div(T * K, kThreads)), dim3(kThreads), 0, st, pos, T * K, row_slot));

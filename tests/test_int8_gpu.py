@@ -747,3 +747,15 @@ def test_results_at_16_byte_aligned_addresses(counts, loose, K, N, swiglu, dtype
                   code, space.data_ptr() + 16, scratch.data_ptr(), n, torch.cuda.current_stream().cuda_stream))
     assert space.data_ptr() % 32 == 0
     assert torch.equal(space[pad:-pad].view(M, N), want) and (space[:pad] == 7).all() and (space[-pad:] == 7).all()
+
+
+def test_codes_into_more_rows_than_the_permutation_takes():
+    """A plan made elsewhere with 40 slots per token: the quantiser has no limit of 32."""
+    T, D, K = 9, 64, 40
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(T, D, generator=g).to(BF16).to(DEV)
+    pos = torch.randperm(T * K, generator=g).to(DEV, torch.int32).view(T, K)
+    plan = bw.PermutePlan(torch.tensor([0, T * K], dtype=torch.int32, device=DEV), pos)
+    codes, s = bw.quantize_tokens_int8(x, plan)
+    alone, scale = bw.quantize_tokens_int8(x)
+    assert torch.equal(codes[pos.long()], alone[:, None].expand(T, K, D)) and torch.equal(s[pos.long()], scale[:, None].expand(T, K))

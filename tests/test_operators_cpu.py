@@ -130,7 +130,7 @@ def test_row_slots_and_negative_expert_counts_are_refused():
     lib, p = bw.lib(), 4096
     bad = lambda rc, code, word: rc == code and word in _lib.last_error()                    # noqa: E731
     assert bad(lib.bwmoe_plan_row_slots(p, 0, 2, p, None), -1, "plan_row_slots")
-    assert bad(lib.bwmoe_plan_row_slots(p, 4, 33, p, None), -4, "plan_row_slots")
+    assert bad(lib.bwmoe_plan_row_slots(p, 4, 0, p, None), -1, "plan_row_slots")
     assert bad(lib.bwmoe_plan_row_slots(p, 2 ** 31 - 1, 1, p, None), -4, "too large")
     assert bad(lib.bwmoe_plan_row_slots(None, 4, 2, p, None), -6, "plan_row_slots")
     assert bad(lib.bwmoe_plan_row_slots(p, 4, 2, None, None), -6, "plan_row_slots")
