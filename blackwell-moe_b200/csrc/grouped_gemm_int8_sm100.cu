@@ -110,7 +110,9 @@ __device__ __forceinline__ void tile_table(const I8Params& p, int tile_rows, int
 }
 
 // K blocks per slice (one warp).  In ns, a slicing takes the longer of all K blocks at the memory's rate (32 KiB of weights in
-// 5.5) and of the longest CTA's blocks (one takes an SM about 500), and then the adding up: fixed, and per slice.
+// 5.5, which is 6 TB/s) and of the longest CTA's blocks, and then the adding up: fixed, and per slice.  One K block of a CTA counts
+// as 500.  Measured, weights from memory, by the difference between K = 32768 and 65536 and between 65536 and 131056: 32-row
+// tiles 260 (64 CTAs) to 320 - 440 (100), 128-row tiles 350 - 450; the rest is for what the others on the chip take of the memory.
 __device__ __forceinline__ int blocks_per_slice(int tiles, int k_blocks, int ctas, int max_pieces, int fixed_ns, int slice_ns) {
   const int lane = threadIdx.x & 31, per = (k_blocks + lane) / (lane + 1), slices = (k_blocks + per - 1) / per;
   const long long pieces = (long long)tiles * slices;
@@ -756,6 +758,8 @@ constexpr size_t kSlabsAt = kArrivalsAt + (S_MAX_PIECES > L_MAX_PIECES ? S_MAX_P
 //   one product, 8 experts of 14336 x 4096:  512 rows each 244 / 208, 1024 rows 356 / 391, 4096 rows 1430 / 1620
 //   SwiGLU:  8 experts of 4096 x 14336, 1024 rows each 800 / 783, 2048 rows 1460 / 1490, 4096 rows 2720 / 2895;
 //     64 experts of 2048 x 1408, 1024 rows each 359 / 336, 2048 rows 580 / 624
+// The borders lie where the two are within 4 % of each other (one product: 67 / 67 at 1024 rows, 201 / 196 and 356 / 391 at 1024
+// rows each; SwiGLU: 1460 / 1490), with one exception: the last line's 2048 rows each (M K N of 3.8e11) get single CTAs.
 bool pair_applies(int M, int K, int N, int E, bool swiglu) {
   if (gemm_sm_budget() < 2) return false;
   if (swiglu) return M >= 2048ll * E && 2.0 * M * K * N >= 4e11;
