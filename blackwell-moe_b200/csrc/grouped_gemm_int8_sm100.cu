@@ -758,8 +758,8 @@ constexpr size_t kSlabsAt = kArrivalsAt + (S_MAX_PIECES > L_MAX_PIECES ? S_MAX_P
 //   one product, 8 experts of 14336 x 4096:  512 rows each 244 / 208, 1024 rows 356 / 391, 4096 rows 1430 / 1620
 //   SwiGLU:  8 experts of 4096 x 14336, 1024 rows each 800 / 783, 2048 rows 1460 / 1490, 4096 rows 2720 / 2895;
 //     64 experts of 2048 x 1408, 1024 rows each 359 / 336, 2048 rows 580 / 624
-// The borders lie where the two are within 4 % of each other (one product: 67 / 67 at 1024 rows, 201 / 196 and 356 / 391 at 1024
-// rows each; SwiGLU: 1460 / 1490), with one exception: the last line's 2048 rows each (M K N of 3.8e11) get single CTAs.
+// At the borders the two are within 4 % of each other (one product: 67 / 67, 149 / 155, 201 / 196; SwiGLU: 1460 / 1490, 359 / 336 just
+// outside).
 bool pair_applies(int M, int K, int N, int E, bool swiglu) {
   if (gemm_sm_budget() < 2) return false;
   if (swiglu) return M >= 2048ll * E && 2.0 * M * K * N >= 4e11;
