@@ -28,7 +28,9 @@ class PermutePlan(NamedTuple):
     ``row_slot[M]``: the slot of each row, ``t*K + k``; ``row_expert[M]``: its expert.  A slot whose expert id is
     outside ``[0, E)`` has no row (``pos`` -1), and the rows past ``offsets[E]`` then have no slot (-1).  The operators
     read ``offsets`` and ``pos`` only: a plan made elsewhere, or one with slots dropped (``pos`` set to -1), may leave the
-    other two out, and may leave any row without a slot.  Two slots never have the same row."""
+    other two out, and may leave any row without a slot.  Two slots never have the same row.  (A plan of this package that
+    was written to without torch counting it, through ``.data`` or by another library, is to be passed as a new
+    ``PermutePlan`` of its tensors.)"""
     offsets: torch.Tensor
     pos: torch.Tensor
     row_slot: Optional[torch.Tensor] = None
@@ -36,9 +38,17 @@ class PermutePlan(NamedTuple):
 
 
 class _OwnPlan(PermutePlan):
-    """A plan as the library wrote it: the rows without a slot are those past ``offsets[E]``."""
+    """A plan as the library wrote it: the rows without a slot are those past ``offsets[E]``.  Copies, of whose tensors nobody
+    knows what they went through, are plain plans, as is what ``_replace`` returns; see :func:`_own_plan`."""
     __slots__ = ()
-    _make = PermutePlan._make           # what _replace() returns is not
+    _make = PermutePlan._make
+
+    def __new__(cls, *args, **kwargs):
+        return PermutePlan(*args, **kwargs)
+
+
+def _own_plan(*tensors):
+    return tuple.__new__(_OwnPlan, tensors)
 
 
 def _is_own(plan) -> bool:
@@ -86,7 +96,7 @@ def _empty_plan(indices, T, K, num_experts, scratch_bytes):
     # (not views of one another: each has its own version, as tensors that were allocated apart)
     o, p, s, e, rest = torch.unsafe_split_with_sizes(indices.new_empty(num_experts + 1 + 3 * M + extra), (num_experts + 1, M, M, M, extra))
     status = rest.data_ptr()
-    return _OwnPlan(o, p.view(T, K), s, e), status, status + 16
+    return _own_plan(o, p.view(T, K), s, e), status, status + 16
 
 
 def _check_indices(indices, num_experts):

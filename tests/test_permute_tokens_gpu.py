@@ -448,3 +448,21 @@ def test_the_librarys_own_plans_need_no_owners():
     assert launches(plan) == 1 and launches(bw.PermutePlan(*plan)) == 2
     plan.pos[3, 1] = -1
     assert launches(plan) == 2
+
+
+def test_copies_of_a_plan_are_plans_from_elsewhere():
+    """Slots dropped, then copied: the copies' tensors are as new, but not as the library wrote them."""
+    import copy
+    import pickle
+    from torch.utils._pytree import tree_map
+    T, D, K = 30, 64, 2
+    idx, _ = routing(T, 8, K, 0)
+    x = torch.randn(T, D, device=DEV)
+    plan = bw.permute_plan(idx.to(DEV), 8)
+    gone = int(plan.pos[3, 1])
+    plan.pos[3, 1] = -1
+    for made in (copy.copy(plan), copy.deepcopy(plan), pickle.loads(pickle.dumps(plan)), tree_map(torch.clone, plan), type(plan)(*[t.clone() for t in plan]),
+                 plan._replace(pos=plan.pos.clone()), type(plan)._make(t.clone() for t in plan)):
+        assert isinstance(made, bw.PermutePlan) and torch.equal(made.pos, plan.pos)
+        rows, back = in_used_memory((T * K, D), F32, lambda: bw.permute_tokens(x, plan=made))
+        assert back is made and (rows[gone] == 0).all() and torch.equal(rows[made.pos[0, 0]], x[0])
