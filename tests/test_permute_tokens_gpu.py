@@ -466,3 +466,34 @@ def test_copies_of_a_plan_are_plans_from_elsewhere():
         assert isinstance(made, bw.PermutePlan) and torch.equal(made.pos, plan.pos)
         rows, back = in_used_memory((T * K, D), F32, lambda: bw.permute_tokens(x, plan=made))
         assert back is made and (rows[gone] == 0).all() and torch.equal(rows[made.pos[0, 0]], x[0])
+
+
+def test_a_captured_step_with_a_plan_from_elsewhere():
+    """Every operator that writes rows, replayed on other places and values: rows without a slot are zeros each time."""
+    T, D, K = 60, 128, 3
+    g = torch.Generator().manual_seed(1)
+
+    def places():
+        pos = torch.randperm(T * K, generator=g).to(torch.int32).view(T, K)
+        return torch.where(torch.rand(T, K, generator=g) < 0.3, -1, pos)
+    plan = bw.PermutePlan(torch.tensor([0, T * K], dtype=torch.int32, device=DEV), places().to(DEV))
+    x, dout = (torch.randn(T, D, generator=g).to(BF16).to(DEV) for _ in range(2))
+    w = torch.rand(T, K, generator=g).to(DEV)
+
+    def step():
+        rows, _ = bw.permute_tokens(x, plan=plan)
+        return (rows, *bw.unpermute_tokens_backward(dout, rows, plan, w), *bw.quantize_tokens_int8(x, plan))
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(3):
+        plan.pos.copy_(places()), x.normal_(), dout.normal_(), w.uniform_()
+        for t in captured:
+            t.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+        free = torch.ones(T * K, dtype=torch.bool, device=DEV)
+        free[plan.pos[plan.pos >= 0].long()] = False
+        assert free.any() and all((t[free] == 0).all() for t in (captured[0], captured[1], captured[3], captured[4]))
